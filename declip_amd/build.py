@@ -11,7 +11,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libdeclip_hip.so")
 STAMP = os.path.join(HERE, "csrc", ".build_stamp")
-BASE_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics", "-Wno-unused-result", "-Wno-unused-value"]
+# no packed fp32 instructions (v_pk_add / mul / fma_f32): the compiler forms them from ordinary float code, and some of their forms have given
+# wrong results on this hardware; two scalar instructions take their place (the host pass does not know the feature and says so)
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+BASE_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics", "-Wno-unused-result", "-Wno-unused-value"] + NO_PACKED_FP32
 FAST_MATH = ["-ffast-math", "-fno-finite-math-only"]
 # Kernels that PRODUCE INDICES (FILIP's top-16 token selection and arg-max bytes, the nearest-neighbour search of the NN bank) are
 # compiled with IEEE arithmetic: a reassociated sum or an approximate reciprocal in a comparison changes WHICH index wins a
