@@ -21,7 +21,9 @@ FAST_MATH = ["-ffast-math", "-fno-finite-math-only"]
 # near-tie, and parity with the reference is judged on exactly those choices (one hardware failure of round 2 was a fast-math
 # reciprocal).  Everything else keeps fast-math (contraction / reassociation inside fp32 epilogues, checked against the oracle
 # at 1e-3).
-IEEE_SOURCES = {"filip.hip", "declip_ops.hip"}
+# The cross-tower operators (xattn / rope / join_norm) are IEEE as well: their bound is memory or the matrix units, and a reassociated sum would only
+# move their results away from the formulas.
+IEEE_SOURCES = {"filip.hip", "declip_ops.hip", "xattn.hip", "rope.hip", "join_norm.hip"}
 FLAGS = BASE_FLAGS + FAST_MATH                 # (the digest below covers both variants)
 
 

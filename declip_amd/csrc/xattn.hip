@@ -1,0 +1,798 @@
+// Cross attention: queries of one packed batch against keys / values of another length (an encoder's states).
+//
+//   s = scale q k^T over the valid keys, p = softmax(s), o = p v;   lse = log sum exp s
+//   D = sum(do o), dv = p^T do, ds = p (do v^T - D), dq = scale ds k, dk = scale ds^T q
+//
+// Rows of one kv head: the `rep` query heads that share it are packed into the query axis, row m = (query m / rep, head m % rep), so
+// shared heads cost no extra pass over k / v and their dk / dv are sums inside one accumulator (a fixed order, no atomics).
+//
+// One pass with running maximum and sum.  The scores are formed TRANSPOSED, S^T = K Q^T (v_mfma 32x32): a lane then owns one query
+// (column), the softmax is in-lane plus one exchange between the half-waves, and the accumulator registers 8t .. 8t+7 of a 32-key block are
+// at once the B operand of the next product O^T = V^T P^T: its contraction index is numbered as the accumulator has it
+// (key 8i + 4h + r <-> slot (h, 4i' + r)), V^T's fragment is read from the row-major tile by the transpose read with the same numbering.
+// P never leaves the registers.
+//   fwd   a wave owns 32 rows m, Q in registers, K / V tiles in LDS
+//   dq    the same with dO in registers too: dP^T = V dO^T, dS^T, dQ^T += K^T dS^T;  writes D for dkv
+//   dkv   a wave owns 32 keys, K / V in registers, Q / dO tiles in LDS: S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS
+// bf16: v_mfma_f32_32x32x16_bf16, P and dS rounded to bf16 as MFMA operands (their sums are formed before, in fp32); fp32:
+// v_mfma_f32_32x32x2_f32, nothing rounded.
+//
+// Keys outside the sequence or masked: their rows are staged as ZEROS (whatever the memory holds, NaN included) and their scores are
+// -inf.  A row without a valid key: o = 0, lse = -inf, no gradient.  Rows that no sequence owns are written as zeros (lse -inf).
+#include "dh_common.h"
+#include <math.h>
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct XP {
+  const void *q, *k, *v, *o, *dout;
+  void *out, *dq, *dk, *dv;
+  float *lse, *delta, *part_o, *part_ml;
+  const int *cu_q, *cu_kv, *kv_len;
+  const uint8_t* key_mask;
+  long ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;
+  int rows_q, rows_kv, batch, heads, kv_heads, rep, hd;
+  float scale;
+  int tiles;          // tiles per (sequence, kv head) in the grid; a block walks t, t + tiles, ... (longer sequences than announced are still whole)
+  int nsplit;         // key ranges per tile (forward)
+  int main_blocks;    // blocks behind these clear the rows no sequence owns
+  int by_pair;        // block order: 1 = the blocks of one (sequence, kv head) on one XCD
+};
+
+template <typename T> struct Op;
+template <> struct Op<bf16_t> {
+  static constexpr int EPC = 8;                      // elements of a 16-byte chunk
+  typedef bf16x8_t Frag;
+  struct PF { bf16x8_t f[2]; };
+  static __device__ __forceinline__ void mma(f32x16_t& c, Frag a, Frag b) { c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ PF pack(const f32x16_t& s) {
+    PF p;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      union { uint32_t u[4]; bf16x8_t v; } x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x.u[e] = pack2bf_hw(s[8 * t + 2 * e], s[8 * t + 2 * e + 1]);
+      p.f[t] = x.v;
+    }
+    return p;
+  }
+  // c[32 columns col0.. of the tile] += tile rows row0 .. row0 + 31, transposed, times p
+  static __device__ __forceinline__ void mma_t(f32x16_t& c, const bf16_t* tile, int ld, int row0, int col0, const PF& p, int lane) {
+    typedef __attribute__((ext_vector_type(4))) short s16x4;
+    const int t16 = lane & 15;
+    const bf16_t* b = tile + (row0 + 4 * (lane >> 5) + (t16 >> 2)) * ld + col0 + 16 * ((lane >> 4) & 1) + 4 * (t16 & 3);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      union { struct { s16x4 a, b; } s; bf16x8_t v; } u;
+      u.s.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(b + (16 * t) * ld));
+      u.s.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(b + (16 * t + 8) * ld));
+      c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u.v, p.f[t], c, 0, 0, 0);
+    }
+  }
+  static __device__ __forceinline__ void store4(bf16_t* p, float a, float b, float c, float d) {
+    uint2 w;
+    w.x = pack2bf_hw(a, b); w.y = pack2bf_hw(c, d);
+    *reinterpret_cast<uint2*>(p) = w;
+  }
+  static __device__ __forceinline__ float dot(Frag a, Frag b) {
+    union { Frag f; uint32_t u[4]; } x, y;
+    x.f = a; y.f = b;
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      s = fmaf(__uint_as_float(x.u[e] << 16), __uint_as_float(y.u[e] << 16), s);
+      s = fmaf(__uint_as_float(x.u[e] & 0xffff0000u), __uint_as_float(y.u[e] & 0xffff0000u), s);
+    }
+    return s;
+  }
+};
+template <> struct Op<float> {
+  static constexpr int EPC = 4;
+  typedef f32x4_t Frag;
+  typedef f32x16_t PF;
+  static __device__ __forceinline__ void mma(f32x16_t& c, Frag a, Frag b) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ PF pack(const f32x16_t& s) { return s; }
+  static __device__ __forceinline__ void mma_t(f32x16_t& c, const float* tile, int ld, int row0, int col0, const PF& p, int lane) {
+    const float* b = tile + (row0 + 4 * (lane >> 5)) * ld + col0 + (lane & 31);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) c = __builtin_amdgcn_mfma_f32_32x32x2f32(b[(8 * i + r) * ld], p[4 * i + r], c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) { *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d); }
+  static __device__ __forceinline__ float dot(Frag a, Frag b) { return fmaf(a[0], b[0], fmaf(a[1], b[1], fmaf(a[2], b[2], a[3] * b[3]))); }
+};
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// ------------------------------------------------------------------------------------------ geometry
+struct Seq { int q0, nq, k0, nk, nseg; };      // query rows, valid keys, key rows of the segment
+__device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); }
+__device__ __forceinline__ Seq seq_of(const XP& p, int b) {
+  Seq s;
+  if (p.cu_q) {
+    s.q0 = clampi(p.cu_q[b], 0, p.rows_q);
+    s.nq = clampi(p.cu_q[b + 1], s.q0, p.rows_q) - s.q0;
+  } else {
+    s.nq = p.rows_q / p.batch;
+    s.q0 = b * s.nq;
+  }
+  if (p.cu_kv) {
+    s.k0 = clampi(p.cu_kv[b], 0, p.rows_kv);
+    s.nseg = clampi(p.cu_kv[b + 1], s.k0, p.rows_kv) - s.k0;
+  } else {
+    s.nseg = p.rows_kv / p.batch;
+    s.k0 = b * s.nseg;
+  }
+  s.nk = p.kv_len ? clampi(p.kv_len[b], 0, s.nseg) : s.nseg;
+  return s;
+}
+
+// block -> (sequence, kv head, tile, split).  by_pair: consecutive blocks go to the 8 XCDs in turn, so the pairs are dealt to the XCDs and all
+// blocks of a pair land on one of them (its L2 then holds that pair's k / v or q / do once).
+struct Work { int b, g, t, split; bool live; };
+__device__ __forceinline__ Work work_of(const XP& p, int bid) {
+  const int inner = p.tiles * p.nsplit, pairs = p.batch * p.kv_heads;
+  int pair, in;
+  if (p.by_pair) {
+    const int slot = bid >> 3;
+    pair = (slot / inner) * 8 + (bid & 7);
+    in = slot % inner;
+  } else {
+    pair = bid / inner;
+    in = bid % inner;
+  }
+  Work w;
+  w.live = pair < pairs;
+  w.g = pair % p.kv_heads;
+  w.b = pair / p.kv_heads;
+  w.split = in % p.nsplit;
+  w.t = in / p.nsplit;
+  return w;
+}
+
+// rows [0, first) and [last, rows) of a [rows][width] matrix are cleared by the blocks behind the main ones
+template <typename T>
+__device__ void clear_rows(T* x, long ld, int width, int first, int last, int rows, int blk, int nblk, int tid, int nthr) {
+  const int nch = width / Op<T>::EPC, n0 = first, n = first + (rows - last);
+  for (long i = (long)blk * nthr + tid; i < (long)n * nch; i += (long)nblk * nthr) {
+    const int r = (int)(i / nch), c = (int)(i % nch);
+    const long row = r < n0 ? r : last + (r - n0);
+    *reinterpret_cast<uint4*>(x + row * ld + (long)c * Op<T>::EPC) = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+__device__ __forceinline__ void owned(const int* cu, int batch, int rows, int& first, int& last) {
+  first = clampi(cu[0], 0, rows);
+  last = clampi(cu[batch], first, rows);
+}
+
+// row m of the packed query axis -> offset of its head's elements
+__device__ __forceinline__ long m_offset(const XP& p, const Seq& s, int g, int m, long ld) {
+  const int q = p.rep == 1 ? m : m / p.rep, r = m - q * p.rep;
+  return (long)(s.q0 + q) * ld + (long)(g * p.rep + r) * p.hd;
+}
+__device__ __forceinline__ long m_stat(const XP& p, const Seq& s, int g, int m) {
+  const int q = p.rep == 1 ? m : m / p.rep, r = m - q * p.rep;
+  return (long)(g * p.rep + r) * p.rows_q + s.q0 + q;
+}
+
+// this lane's operand chunks of one row (lane half h: elements ks * 2 EPC + h EPC ..), zero where dead
+template <typename T, int HDP>
+__device__ __forceinline__ void load_row(typename Op<T>::Frag* f, const T* row, bool live, int hd, int h) {
+  constexpr int EPC = Op<T>::EPC, KS = HDP / (2 * EPC);
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    union { uint4 u; typename Op<T>::Frag f; } x;
+    x.u = make_uint4(0u, 0u, 0u, 0u);
+    const int c = ks * 2 * EPC + h * EPC;
+    if (live && c < hd) x.u = *reinterpret_cast<const uint4*>(row + c);
+    f[ks] = x.f;
+  }
+}
+template <typename T, int HDP>
+__device__ __forceinline__ f32x16_t mma_row(const T* tile, int ld, int row0, const typename Op<T>::Frag* f, int lane) {
+  constexpr int EPC = Op<T>::EPC, KS = HDP / (2 * EPC);
+  f32x16_t c;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) c[i] = 0.f;
+  const T* row = tile + (row0 + (lane & 31)) * ld + (lane >> 5) * EPC;
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) Op<T>::mma(c, *reinterpret_cast<const typename Op<T>::Frag*>(row + ks * 2 * EPC), f[ks]);
+  return c;
+}
+
+// two tiles of ROWS rows on their way from memory to LDS (registers in between)
+template <typename T, int HDP, int ROWS, int NT>
+struct Pair2 {
+  static constexpr int EPC = Op<T>::EPC, NCH = HDP / EPC, N = (ROWS * NCH + NT - 1) / NT, LD = HDP + EPC;
+  uint4 a[N], b[N];
+  // fa(row) / fb(row): element pointers of a tile row, or nullptr for a row of zeros
+  template <typename FA, typename FB>
+  __device__ __forceinline__ void fetch(FA fa, FB fb, int hd, int tid) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int task = tid + k * NT, row = task / NCH, c = task % NCH;
+      a[k] = b[k] = make_uint4(0u, 0u, 0u, 0u);
+      if (ROWS * NCH % NT != 0 && task >= ROWS * NCH) continue;
+      if (c * EPC < hd) {
+        const T *pa = fa(row), *pb = fb(row);
+        if (pa) { a[k] = *reinterpret_cast<const uint4*>(pa + c * EPC); b[k] = *reinterpret_cast<const uint4*>(pb + c * EPC); }
+      }
+    }
+  }
+  template <typename FD>
+  __device__ __forceinline__ void store(T* ta, T* tb, FD dead, int tid) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int task = tid + k * NT, row = task / NCH, c = task % NCH;
+      if (ROWS * NCH % NT != 0 && task >= ROWS * NCH) continue;
+      if (dead(row)) a[k] = b[k] = make_uint4(0u, 0u, 0u, 0u);
+      *reinterpret_cast<uint4*>(ta + row * LD + c * EPC) = a[k];
+      *reinterpret_cast<uint4*>(tb + row * LD + c * EPC) = b[k];
+    }
+  }
+};
+
+// ------------------------------------------------------------------------------------------ forward
+template <typename T, int HDP, int NW, int BN, bool SPLIT>
+__global__ __launch_bounds__(64 * NW) void xattn_fwd_kernel(XP p) {
+  constexpr int EPC = Op<T>::EPC, LD = HDP + EPC, KS = HDP / (2 * EPC), DB = HDP / 32, NB = BN / 32, BM = 32 * NW, NT = 64 * NW;
+  DH_DYN_LDS_A16(unsigned char, smem);
+  T* Ks = reinterpret_cast<T*>(smem);
+  T* Vs = Ks + BN * LD;
+  float* bias = reinterpret_cast<float*>(Vs + BN * LD);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+  const T *q = (const T*)p.q, *kp = (const T*)p.k, *vp = (const T*)p.v;
+  if ((int)blockIdx.x >= p.main_blocks) {
+    int first, last;
+    owned(p.cu_q, p.batch, p.rows_q, first, last);
+    const int blk = blockIdx.x - p.main_blocks, nblk = gridDim.x - p.main_blocks;
+    clear_rows<T>((T*)p.out, p.ldo, p.heads * p.hd, first, last, p.rows_q, blk, nblk, tid, NT);
+    const int n = first + p.rows_q - last;
+    for (long i = (long)blk * NT + tid; i < (long)n * p.heads; i += (long)nblk * NT) {
+      const int r = (int)(i % n);
+      p.lse[(i / n) * p.rows_q + (r < first ? r : last + r - first)] = -INFINITY;
+    }
+    return;
+  }
+  const Work w = work_of(p, blockIdx.x);
+  if (!w.live) return;
+  const Seq s = seq_of(p, w.b);
+  const int M = s.nq * p.rep;
+  const int nt = (s.nk + BN - 1) / BN;
+  int lo = 0, hi = nt;
+  if (SPLIT) {
+    const int per = (nt + p.nsplit - 1) / p.nsplit;
+    lo = min(w.split * per, nt);
+    hi = min(lo + per, nt);
+  }
+  const float c = p.scale * kLog2e;
+  const uint8_t* km = p.key_mask ? p.key_mask + s.k0 : nullptr;
+  const T* kb_ = kp + (long)s.k0 * p.ldk + (long)w.g * p.hd;
+  const T* vb_ = vp + (long)s.k0 * p.ldv + (long)w.g * p.hd;
+
+  for (int t = w.t; (long)t * BM < M; t += p.tiles) {
+    const int m = t * BM + wave * 32 + (lane & 31);
+    const bool live = m < M, wave_live = t * BM + wave * 32 < M;
+    typename Op<T>::Frag qf[KS];
+    load_row<T, HDP>(qf, q + (live ? m_offset(p, s, w.g, m, p.ldq) : 0), live, p.hd, h);
+    f32x16_t o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+    float mrun = -INFINITY, l = 0.f;
+    Pair2<T, HDP, BN, NT> st;
+    auto fetch = [&](int kt) {
+      st.fetch([&](int r) -> const T* { const int key = kt * BN + r; return key < s.nk ? kb_ + (long)key * p.ldk : nullptr; },
+               [&](int r) -> const T* { return vb_ + (long)(kt * BN + r) * p.ldv; }, p.hd, tid);
+    };
+    if (lo < hi) fetch(lo);
+    for (int kt = lo; kt < hi; ++kt) {
+      __syncthreads();                               // the tile before is read
+      st.store(Ks, Vs, [&](int r) { const int key = kt * BN + r; return km != nullptr && key < s.nk && !km[key]; }, tid);
+      const bool masked = km != nullptr || (kt + 1) * BN > s.nk;
+      if (masked)
+        for (int r = tid; r < BN; r += NT) {
+          const int key = kt * BN + r;
+          bias[r] = key < s.nk && (!km || km[key]) ? 0.f : -INFINITY;
+        }
+      __syncthreads();
+      if (kt + 1 < hi) fetch(kt + 1);
+      if (!wave_live) continue;
+      f32x16_t sc[NB];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) sc[b] = mma_row<T, HDP>(Ks, LD, b * 32, qf, lane);
+      if (masked) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float4 bi = *reinterpret_cast<const float4*>(bias + b * 32 + 8 * i + 4 * h);
+            // (a select, not a sum: a masked score may be anything)
+            sc[b][4 * i] = bi.x < 0.f ? -INFINITY : sc[b][4 * i]; sc[b][4 * i + 1] = bi.y < 0.f ? -INFINITY : sc[b][4 * i + 1];
+            sc[b][4 * i + 2] = bi.z < 0.f ? -INFINITY : sc[b][4 * i + 2]; sc[b][4 * i + 3] = bi.w < 0.f ? -INFINITY : sc[b][4 * i + 3];
+          }
+      }
+      float mx = sc[0][0];
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[b][i]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float mnew = fmaxf(mrun, mx * c), ms = mnew == -INFINITY ? 0.f : mnew;
+      const float alpha = exp2_fast(mrun - ms);
+      mrun = mnew;
+      float sum = 0.f;
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float e = exp2_fast(fmaf(sc[b][i], c, -ms));
+          sc[b][i] = e;
+          sum += e;
+        }
+      l = fmaf(l, alpha, sum);                       // this half-wave's keys; joined behind the loop
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const typename Op<T>::PF pf = Op<T>::pack(sc[b]);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) Op<T>::mma_t(o[d], Vs, LD, b * 32, d * 32, pf, lane);
+      }
+    }
+    l += __shfl_xor(l, 32, 64);
+    if (live) {
+      const long stat = m_stat(p, s, w.g, m);
+      if (SPLIT) {
+        const long part = (long)w.split * p.heads * p.rows_q + stat;
+        if (h == 0) { p.part_ml[2 * part] = mrun; p.part_ml[2 * part + 1] = l; }
+        if (lo < hi) {
+#pragma unroll
+          for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int col = d * 32 + 8 * i + 4 * h;
+              if (col < p.hd)
+                *reinterpret_cast<float4*>(p.part_o + part * p.hd + col) = make_float4(o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]);
+            }
+        }
+      } else {
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+        if (h == 0) p.lse[stat] = l == 0.f ? -INFINITY : (mrun + __log2f(l)) * kLn2;
+        T* orow = (T*)p.out + m_offset(p, s, w.g, m, p.ldo);
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int col = d * 32 + 8 * i + 4 * h;
+            if (col < p.hd) Op<T>::store4(orow + col, o[d][4 * i] * inv, o[d][4 * i + 1] * inv, o[d][4 * i + 2] * inv, o[d][4 * i + 3] * inv);
+          }
+      }
+    }
+  }
+}
+
+// joins the key ranges of one (query row, head): o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, ranges in ascending order
+template <typename T>
+__global__ __launch_bounds__(256) void xattn_join_kernel(XP p) {
+  int first = 0, last = p.rows_q;
+  if (p.cu_q) owned(p.cu_q, p.batch, p.rows_q, first, last);
+  const int lane = threadIdx.x & 63;
+  const long n = (long)(last - first) * p.heads, stride = (long)p.heads * p.rows_q;
+  for (long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += (long)gridDim.x * 4) {
+    const int row = first + (int)(i / p.heads), head = (int)(i % p.heads);
+    const long stat = (long)head * p.rows_q + row;
+    float m = -INFINITY;
+    for (int s = 0; s < p.nsplit; ++s) m = fmaxf(m, p.part_ml[2 * (s * stride + stat)]);
+    const float ms = m == -INFINITY ? 0.f : m;
+    float l = 0.f, a0 = 0.f, a1 = 0.f;
+    for (int s = 0; s < p.nsplit; ++s) {
+      const long part = s * stride + stat;
+      const float ml = p.part_ml[2 * part + 1];
+      if (ml == 0.f) continue;                       // an empty range wrote no sums
+      const float f = exp2_fast(p.part_ml[2 * part] - ms);
+      l = fmaf(f, ml, l);
+      if (lane < p.hd) a0 = fmaf(f, p.part_o[part * p.hd + lane], a0);
+      if (lane + 64 < p.hd) a1 = fmaf(f, p.part_o[part * p.hd + lane + 64], a1);
+    }
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    T* o = (T*)p.out + (long)row * p.ldo + (long)head * p.hd;
+    if (lane < p.hd) st<T>(o + lane, a0 * inv);
+    if (lane + 64 < p.hd) st<T>(o + lane + 64, a1 * inv);
+    if (lane == 0) p.lse[stat] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
+  }
+}
+
+// ------------------------------------------------------------------------------------------ backward: dq (and D)
+template <typename T, int HDP, int NW, int BN>
+__global__ __launch_bounds__(64 * NW) void xattn_dq_kernel(XP p) {
+  constexpr int EPC = Op<T>::EPC, LD = HDP + EPC, KS = HDP / (2 * EPC), DB = HDP / 32, NB = BN / 32, BM = 32 * NW, NT = 64 * NW;
+  DH_DYN_LDS_A16(unsigned char, smem);
+  T* Ks = reinterpret_cast<T*>(smem);
+  T* Vs = Ks + BN * LD;
+  float* bias = reinterpret_cast<float*>(Vs + BN * LD);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+  if ((int)blockIdx.x >= p.main_blocks) {
+    int first, last;
+    owned(p.cu_q, p.batch, p.rows_q, first, last);
+    clear_rows<T>((T*)p.dq, p.lddq, p.heads * p.hd, first, last, p.rows_q, blockIdx.x - p.main_blocks, gridDim.x - p.main_blocks, tid, NT);
+    return;
+  }
+  const Work w = work_of(p, blockIdx.x);
+  if (!w.live) return;
+  const Seq s = seq_of(p, w.b);
+  const int M = s.nq * p.rep, nt = (s.nk + BN - 1) / BN;
+  const float c = p.scale * kLog2e;
+  const uint8_t* km = p.key_mask ? p.key_mask + s.k0 : nullptr;
+  const T* kb_ = (const T*)p.k + (long)s.k0 * p.ldk + (long)w.g * p.hd;
+  const T* vb_ = (const T*)p.v + (long)s.k0 * p.ldv + (long)w.g * p.hd;
+  for (int t = w.t; (long)t * BM < M; t += p.tiles) {
+    const int m = t * BM + wave * 32 + (lane & 31);
+    const bool live = m < M, wave_live = t * BM + wave * 32 < M;
+    const long stat = live ? m_stat(p, s, w.g, m) : 0;
+    const float lse = live ? p.lse[stat] : -INFINITY;
+    const bool has = live && lse != -INFINITY;       // a row without a key: no gradient, whatever do holds
+    const float lse2 = has ? lse * kLog2e : INFINITY;
+    typename Op<T>::Frag qf[KS], df[KS];
+    load_row<T, HDP>(qf, (const T*)p.q + (has ? m_offset(p, s, w.g, m, p.ldq) : 0), has, p.hd, h);
+    load_row<T, HDP>(df, (const T*)p.dout + (has ? m_offset(p, s, w.g, m, p.lddo) : 0), has, p.hd, h);
+    float D = 0.f;
+    {
+      typename Op<T>::Frag of[KS];
+      load_row<T, HDP>(of, (const T*)p.o + (has ? m_offset(p, s, w.g, m, p.ldo) : 0), has, p.hd, h);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) D += Op<T>::dot(df[ks], of[ks]);
+    }
+    D += __shfl_xor(D, 32, 64);
+    if (live && h == 0) p.delta[stat] = D;
+    f32x16_t dq[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dq[d][i] = 0.f;
+    Pair2<T, HDP, BN, NT> st;
+    auto fetch = [&](int kt) {
+      st.fetch([&](int r) -> const T* { const int key = kt * BN + r; return key < s.nk ? kb_ + (long)key * p.ldk : nullptr; },
+               [&](int r) -> const T* { return vb_ + (long)(kt * BN + r) * p.ldv; }, p.hd, tid);
+    };
+    if (nt > 0) fetch(0);
+    for (int kt = 0; kt < nt; ++kt) {
+      __syncthreads();
+      st.store(Ks, Vs, [&](int r) { const int key = kt * BN + r; return km != nullptr && key < s.nk && !km[key]; }, tid);
+      const bool masked = km != nullptr || (kt + 1) * BN > s.nk;
+      if (masked)
+        for (int r = tid; r < BN; r += NT) {
+          const int key = kt * BN + r;
+          bias[r] = key < s.nk && (!km || km[key]) ? 0.f : -INFINITY;
+        }
+      __syncthreads();
+      if (kt + 1 < nt) fetch(kt + 1);
+      if (!wave_live) continue;
+      auto p_dp = [&](int b, f32x16_t& sc, f32x16_t& dp) {       // p and dp of 32 keys
+        sc = mma_row<T, HDP>(Ks, LD, b * 32, qf, lane);
+        dp = mma_row<T, HDP>(Vs, LD, b * 32, df, lane);
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float4 bi = *reinterpret_cast<const float4*>(bias + b * 32 + 8 * i + 4 * h);
+            sc[4 * i] = bi.x < 0.f ? -INFINITY : sc[4 * i]; sc[4 * i + 1] = bi.y < 0.f ? -INFINITY : sc[4 * i + 1];
+            sc[4 * i + 2] = bi.z < 0.f ? -INFINITY : sc[4 * i + 2]; sc[4 * i + 3] = bi.w < 0.f ? -INFINITY : sc[4 * i + 3];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[i] = exp2_fast(fmaf(sc[i], c, -lse2));
+      };
+      if (sizeof(T) == 2 && nt == 1) {
+        // all keys are here: D = sum p dp, which is sum(do o) before o was rounded.  With a few keys dp - D cancels, and the rounding of o
+        // alone would double the error of dq and dk (two keys: 3.6e-3 instead of 2.4e-3 of their norm); over many keys |o| is small against |v|.
+        D = 0.f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          f32x16_t sc, dp;
+          p_dp(b, sc, dp);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) D = fmaf(sc[i], dp[i], D);
+        }
+        D += __shfl_xor(D, 32, 64);
+        if (live && h == 0) p.delta[stat] = D;
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        f32x16_t sc, dp;
+        p_dp(b, sc, dp);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[i] *= dp[i] - D;
+        const typename Op<T>::PF pf = Op<T>::pack(sc);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) Op<T>::mma_t(dq[d], Ks, LD, b * 32, d * 32, pf, lane);
+      }
+    }
+    if (live) {
+      T* row = (T*)p.dq + m_offset(p, s, w.g, m, p.lddq);
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int col = d * 32 + 8 * i + 4 * h;
+          if (col < p.hd) Op<T>::store4(row + col, dq[d][4 * i] * p.scale, dq[d][4 * i + 1] * p.scale, dq[d][4 * i + 2] * p.scale, dq[d][4 * i + 3] * p.scale);
+        }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------ backward: dk, dv
+template <typename T, int HDP, int NW, int BQ>
+__global__ __launch_bounds__(64 * NW) void xattn_dkv_kernel(XP p) {
+  constexpr int EPC = Op<T>::EPC, LD = HDP + EPC, KS = HDP / (2 * EPC), DB = HDP / 32, NB = BQ / 32, BK = 32 * NW, NT = 64 * NW;
+  DH_DYN_LDS_A16(unsigned char, smem);
+  T* Qs = reinterpret_cast<T*>(smem);
+  T* Ds = Qs + BQ * LD;
+  float* lse2s = reinterpret_cast<float*>(Ds + BQ * LD);
+  float* dels = lse2s + BQ;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+  if ((int)blockIdx.x >= p.main_blocks) {
+    int first, last;
+    owned(p.cu_kv, p.batch, p.rows_kv, first, last);
+    const int blk = blockIdx.x - p.main_blocks, nblk = gridDim.x - p.main_blocks;
+    clear_rows<T>((T*)p.dk, p.lddk, p.kv_heads * p.hd, first, last, p.rows_kv, blk, nblk, tid, NT);
+    clear_rows<T>((T*)p.dv, p.lddv, p.kv_heads * p.hd, first, last, p.rows_kv, blk, nblk, tid, NT);
+    return;
+  }
+  const Work w = work_of(p, blockIdx.x);
+  if (!w.live) return;
+  const Seq s = seq_of(p, w.b);
+  const int M = s.nq * p.rep, nt = (M + BQ - 1) / BQ;
+  const float c = p.scale * kLog2e;
+  for (int t = w.t; (long)t * BK < s.nseg; t += p.tiles) {
+    const int key = t * BK + wave * 32 + (lane & 31);
+    const bool in = key < s.nseg, live = key < s.nk && (!p.key_mask || p.key_mask[s.k0 + key]);
+    const bool wave_live = t * BK + wave * 32 < s.nk, block_live = t * BK < s.nk;
+    typename Op<T>::Frag kf[KS], vf[KS];
+    load_row<T, HDP>(kf, (const T*)p.k + (live ? (long)(s.k0 + key) * p.ldk + (long)w.g * p.hd : 0), live, p.hd, h);
+    load_row<T, HDP>(vf, (const T*)p.v + (live ? (long)(s.k0 + key) * p.ldv + (long)w.g * p.hd : 0), live, p.hd, h);
+    f32x16_t dk[DB], dv[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dk[d][i] = dv[d][i] = 0.f;
+    Pair2<T, HDP, BQ, NT> st;
+    auto fetch = [&](int mt) {
+      st.fetch([&](int r) -> const T* { const int m = mt * BQ + r; return m < M ? (const T*)p.q + m_offset(p, s, w.g, m, p.ldq) : nullptr; },
+               [&](int r) -> const T* { return (const T*)p.dout + m_offset(p, s, w.g, mt * BQ + r, p.lddo); }, p.hd, tid);
+    };
+    const int n_mt = block_live ? nt : 0;
+    if (n_mt > 0) fetch(0);
+    for (int mt = 0; mt < n_mt; ++mt) {
+      __syncthreads();
+      st.store(Qs, Ds, [](int) { return false; }, tid);
+      for (int r = tid; r < BQ; r += NT) {
+        const int m = mt * BQ + r;
+        float a = INFINITY, d = 0.f;
+        if (m < M) {
+          const long stat = m_stat(p, s, w.g, m);
+          const float lse = p.lse[stat];
+          a = lse == -INFINITY ? INFINITY : lse * kLog2e;
+          d = p.delta[stat];
+        }
+        lse2s[r] = a;
+        dels[r] = d;
+      }
+      __syncthreads();
+      if (mt + 1 < n_mt) fetch(mt + 1);
+      if (!wave_live) continue;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        f32x16_t sc = mma_row<T, HDP>(Qs, LD, b * 32, kf, lane);
+        f32x16_t dp = mma_row<T, HDP>(Ds, LD, b * 32, vf, lane);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float4 L = *reinterpret_cast<const float4*>(lse2s + b * 32 + 8 * i + 4 * h);
+          const float4 D = *reinterpret_cast<const float4*>(dels + b * 32 + 8 * i + 4 * h);
+          sc[4 * i] = exp2_fast(fmaf(sc[4 * i], c, -L.x)); dp[4 * i] = sc[4 * i] * (dp[4 * i] - D.x);
+          sc[4 * i + 1] = exp2_fast(fmaf(sc[4 * i + 1], c, -L.y)); dp[4 * i + 1] = sc[4 * i + 1] * (dp[4 * i + 1] - D.y);
+          sc[4 * i + 2] = exp2_fast(fmaf(sc[4 * i + 2], c, -L.z)); dp[4 * i + 2] = sc[4 * i + 2] * (dp[4 * i + 2] - D.z);
+          sc[4 * i + 3] = exp2_fast(fmaf(sc[4 * i + 3], c, -L.w)); dp[4 * i + 3] = sc[4 * i + 3] * (dp[4 * i + 3] - D.w);
+        }
+        const typename Op<T>::PF pf = Op<T>::pack(sc), sf = Op<T>::pack(dp);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          Op<T>::mma_t(dv[d], Ds, LD, b * 32, d * 32, pf, lane);
+          Op<T>::mma_t(dk[d], Qs, LD, b * 32, d * 32, sf, lane);
+        }
+      }
+    }
+    if (in) {
+      T* krow = (T*)p.dk + (long)(s.k0 + key) * p.lddk + (long)w.g * p.hd;
+      T* vrow = (T*)p.dv + (long)(s.k0 + key) * p.lddv + (long)w.g * p.hd;
+      // (a masked key's column may hold anything: it is written as zeros)
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int col = d * 32 + 8 * i + 4 * h;
+          if (col >= p.hd) continue;
+          float a[4], b[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) { a[r] = live ? dk[d][4 * i + r] * p.scale : 0.f; b[r] = live ? dv[d][4 * i + r] : 0.f; }
+          Op<T>::store4(krow + col, a[0], a[1], a[2], a[3]);
+          Op<T>::store4(vrow + col, b[0], b[1], b[2], b[3]);
+        }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------ host side
+int x_cus() {
+  static int n = 0;
+  if (!n) {
+    int dev = 0;
+    hipDeviceProp_t pr;
+    n = (hipGetDevice(&dev) == hipSuccess && hipGetDeviceProperties(&pr, dev) == hipSuccess && pr.multiProcessorCount > 0) ? pr.multiProcessorCount : 256;
+  }
+  return n;
+}
+
+int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// longest length to lay the grid out for: the caller's bound, or twice the mean of a packed batch (longer ones take several rounds)
+int length_hint(int given, const int* cu, int rows, int batch) {
+  if (!cu) return rows / batch;
+  int64_t n = given > 0 ? given : 2 * cdiv64(rows, batch);
+  return (int)(n > rows ? rows : n);
+}
+
+struct Plan { int nw, bn, tiles, nsplit; };
+Plan plan_fwd(const dh_xattn_args* a) {
+  const int rep = a->heads / a->kv_heads;
+  const int64_t mq = (int64_t)length_hint(a->max_q, a->cu_q, a->rows_q, a->batch) * rep;
+  const int mk = length_hint(a->max_kv, a->cu_kv, a->rows_kv, a->batch);
+  Plan r;
+  r.nw = mq <= 32 ? 1 : 4;
+  r.bn = (r.nw == 1 || a->dtype == DH_F32) ? 32 : 64;
+  r.tiles = (int)cdiv64(mq < 1 ? 1 : mq, 32 * r.nw);
+  const int64_t blocks = (int64_t)r.tiles * a->batch * a->kv_heads, want = (int64_t)x_cus() * (r.nw == 1 ? 8 : 2);
+  int64_t ns = blocks >= want ? 1 : want / blocks;
+  const int64_t most = cdiv64(mk, 4 * r.bn);          // a range is at least four tiles long
+  if (ns > most) ns = most;
+  if (ns > 64) ns = 64;
+  r.nsplit = ns < 1 ? 1 : (int)ns;
+  return r;
+}
+
+int check_args(const dh_xattn_args* a, const char* who, bool bwd) {
+  DH_REQUIRE(a, "%s: null args", who);
+  DH_REQUIRE(a->dtype == DH_F32 || a->dtype == DH_BF16, "%s: dtype %d", who, a->dtype);
+  DH_REQUIRE(a->batch > 0 && a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0, "%s: batch %d, heads %d, kv_heads %d", who, a->batch, a->heads, a->kv_heads);
+  DH_REQUIRE(a->hd >= 8 && a->hd <= 128 && a->hd % 8 == 0, "%s: head size %d (a multiple of 8 up to 128)", who, a->hd);
+  DH_REQUIRE(a->rows_q >= 0 && a->rows_kv >= 0, "%s: negative row count", who);
+  DH_REQUIRE(a->cu_q || a->rows_q % a->batch == 0, "%s: %d query rows do not divide into %d sequences", who, a->rows_q, a->batch);
+  DH_REQUIRE(a->cu_kv || a->rows_kv % a->batch == 0, "%s: %d key rows do not divide into %d sequences", who, a->rows_kv, a->batch);
+  DH_REQUIRE(a->scale > 0.f && a->scale < INFINITY, "%s: scale must be positive and finite", who);
+  DH_REQUIRE((int64_t)a->rows_q * (a->heads / a->kv_heads) < (1ll << 30) && a->rows_kv < (1 << 30), "%s: too many rows", who);
+  const int epc = a->dtype == DH_BF16 ? 8 : 4;
+  const int64_t wq = (int64_t)a->heads * a->hd, wk = (int64_t)a->kv_heads * a->hd;
+  struct { const void* p; int64_t ld, w; bool need; const char* name; } m[] = {
+      {a->q, a->ldq, wq, a->rows_q > 0, "q"},       {a->k, a->ldk, wk, a->rows_kv > 0, "k"},          {a->v, a->ldv, wk, a->rows_kv > 0, "v"},
+      {a->out, a->ldo, wq, a->rows_q > 0, "out"},   {a->dout, a->lddo, wq, bwd && a->rows_q > 0, "dout"}, {a->dq, a->lddq, wq, bwd && a->rows_q > 0, "dq"},
+      {a->dk, a->lddk, wk, bwd && a->rows_kv > 0, "dk"}, {a->dv, a->lddv, wk, bwd && a->rows_kv > 0, "dv"}};
+  for (const auto& x : m) {
+    if (!x.need) continue;
+    DH_REQUIRE(x.p, "%s: %s is NULL", who, x.name);
+    DH_REQUIRE(((uintptr_t)x.p & 15) == 0 && x.ld >= x.w && x.ld % epc == 0, "%s: %s needs 16-byte aligned rows (row stride %lld, width %lld)", who, x.name,
+               (long long)x.ld, (long long)x.w);
+  }
+  DH_REQUIRE(a->lse || a->rows_q == 0, "%s: lse is NULL", who);
+  return DH_OK;
+}
+
+XP params(const dh_xattn_args* a) {
+  XP p = {};
+  p.q = a->q; p.k = a->k; p.v = a->v; p.o = a->out; p.dout = a->dout;
+  p.out = a->out; p.dq = a->dq; p.dk = a->dk; p.dv = a->dv; p.lse = a->lse;
+  p.cu_q = a->cu_q; p.cu_kv = a->cu_kv; p.kv_len = a->kv_len; p.key_mask = a->key_mask;
+  p.ldq = a->ldq; p.ldk = a->ldk; p.ldv = a->ldv; p.ldo = a->ldo; p.lddo = a->lddo; p.lddq = a->lddq; p.lddk = a->lddk; p.lddv = a->lddv;
+  p.rows_q = a->rows_q; p.rows_kv = a->rows_kv; p.batch = a->batch; p.heads = a->heads; p.kv_heads = a->kv_heads; p.rep = a->heads / a->kv_heads; p.hd = a->hd;
+  p.scale = a->scale;
+  p.nsplit = 1;
+  return p;
+}
+
+// grid of a kernel over (sequence, kv head) pairs; `clear`: blocks behind it for the rows no sequence owns
+int lay_out(XP& p, int tiles, int nsplit, bool clear, int64_t& grid) {
+  const int64_t pairs = (int64_t)p.batch * p.kv_heads;
+  p.tiles = tiles < 1 ? 1 : tiles;
+  p.nsplit = nsplit;
+  p.by_pair = pairs % 8 == 0 || pairs >= 64;
+  const int64_t main = (p.by_pair ? cdiv64(pairs, 8) * 8 : pairs) * p.tiles * nsplit;
+  DH_REQUIRE(main < (1ll << 30), "dh_xattn: grid of %lld blocks", (long long)main);
+  p.main_blocks = (int)main;
+  grid = main + (clear ? 64 : 0);
+  return DH_OK;
+}
+
+template <typename K>
+int launch(K kernel, const XP& p, int64_t grid, int threads, size_t lds, hipStream_t st) {
+  if (lds > 64 * 1024) DH_RT(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), "hipFuncSetAttribute");
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(threads), lds, st, p);
+  DH_CHECK_LAUNCH();
+  return DH_OK;
+}
+
+template <typename T, int HDP> constexpr size_t tile_bytes(int rows) { return (size_t)2 * rows * (HDP + Op<T>::EPC) * sizeof(T); }
+
+template <typename T, int HDP>
+int fwd_hd(XP& p, const Plan& pl, int64_t grid, hipStream_t st) {
+  constexpr int BN = sizeof(T) == 2 ? 64 : 32;
+  const size_t lds1 = tile_bytes<T, HDP>(32) + 32 * 4, lds4 = tile_bytes<T, HDP>(BN) + BN * 4;
+  if (pl.nw == 1) return pl.nsplit > 1 ? launch(xattn_fwd_kernel<T, HDP, 1, 32, true>, p, grid, 64, lds1, st) : launch(xattn_fwd_kernel<T, HDP, 1, 32, false>, p, grid, 64, lds1, st);
+  return pl.nsplit > 1 ? launch(xattn_fwd_kernel<T, HDP, 4, BN, true>, p, grid, 256, lds4, st) : launch(xattn_fwd_kernel<T, HDP, 4, BN, false>, p, grid, 256, lds4, st);
+}
+template <typename T, int HDP>
+int bwd_hd(XP& p, const dh_xattn_args* a, hipStream_t st) {
+  constexpr int BN = sizeof(T) == 2 ? 64 : 32;
+  int64_t grid;
+  const int64_t mq = (int64_t)length_hint(a->max_q, a->cu_q, a->rows_q, a->batch) * p.rep;
+  if (a->rows_q > 0) {
+    if (int e = lay_out(p, (int)cdiv64(mq, 128), 1, a->cu_q != nullptr, grid)) return e;
+    if (int e = launch(xattn_dq_kernel<T, HDP, 4, BN>, p, grid, 256, tile_bytes<T, HDP>(BN) + BN * 4, st)) return e;
+  }
+  if (a->rows_kv > 0) {
+    if (int e = lay_out(p, (int)cdiv64(length_hint(a->max_kv, a->cu_kv, a->rows_kv, a->batch), 128), 1, a->cu_kv != nullptr, grid)) return e;
+    if (int e = launch(xattn_dkv_kernel<T, HDP, 4, 32>, p, grid, 256, tile_bytes<T, HDP>(32) + 32 * 8, st)) return e;
+  }
+  return DH_OK;
+}
+
+#define XATTN_HD(fn, T, ...) \
+  (p.hd <= 32 ? fn<T, 32>(__VA_ARGS__) : p.hd <= 64 ? fn<T, 64>(__VA_ARGS__) : p.hd <= 96 ? fn<T, 96>(__VA_ARGS__) : fn<T, 128>(__VA_ARGS__))
+
+int64_t split_bytes(const dh_xattn_args* a, int nsplit) { return nsplit > 1 ? (int64_t)nsplit * a->heads * a->rows_q * (a->hd + 2) * 4 : 0; }
+
+}  // namespace
+
+extern "C" int64_t dh_xattn_ws_bytes(const dh_xattn_args* a, int backward) {
+  if (check_args(a, "dh_xattn_ws_bytes", false) == DH_ERR_ARG && (!a || a->batch <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->heads % a->kv_heads != 0)) return -1;
+  if (backward) return (int64_t)a->heads * a->rows_q * 4;
+  return split_bytes(a, plan_fwd(a).nsplit);
+}
+
+extern "C" int dh_xattn_fwd(const dh_xattn_args* a, dh_stream_t stream) {
+  if (int e = check_args(a, "dh_xattn_fwd", false)) return e;
+  if (a->rows_q == 0) return DH_OK;
+  const Plan pl = plan_fwd(a);
+  XP p = params(a);
+  const int64_t need = split_bytes(a, pl.nsplit);
+  DH_REQUIRE(need == 0 || (a->ws && a->ws_bytes >= need && ((uintptr_t)a->ws & 15) == 0), "dh_xattn_fwd: workspace of %lld bytes needed", (long long)need);
+  if (need) {
+    p.part_o = (float*)a->ws;
+    p.part_ml = p.part_o + (int64_t)pl.nsplit * a->heads * a->rows_q * a->hd;
+  }
+  int64_t grid;
+  if (int e = lay_out(p, pl.tiles, pl.nsplit, a->cu_q != nullptr, grid)) return e;
+  const int rc = a->dtype == DH_BF16 ? XATTN_HD(fwd_hd, bf16_t, p, pl, grid, (hipStream_t)stream) : XATTN_HD(fwd_hd, float, p, pl, grid, (hipStream_t)stream);
+  if (rc || pl.nsplit == 1) return rc;
+  int64_t jg = cdiv64((int64_t)a->rows_q * a->heads, 4);
+  if (jg > 8 * x_cus()) jg = 8 * x_cus();
+  if (a->dtype == DH_BF16) hipLaunchKernelGGL(xattn_join_kernel<bf16_t>, dim3((unsigned)jg), dim3(256), 0, (hipStream_t)stream, p);
+  else hipLaunchKernelGGL(xattn_join_kernel<float>, dim3((unsigned)jg), dim3(256), 0, (hipStream_t)stream, p);
+  DH_CHECK_LAUNCH();
+  return DH_OK;
+}
+
+extern "C" int dh_xattn_bwd(const dh_xattn_args* a, dh_stream_t stream) {
+  if (int e = check_args(a, "dh_xattn_bwd", true)) return e;
+  const int64_t need = (int64_t)a->heads * a->rows_q * 4;
+  DH_REQUIRE(need == 0 || (a->ws && a->ws_bytes >= need && ((uintptr_t)a->ws & 15) == 0), "dh_xattn_bwd: workspace of %lld bytes needed", (long long)need);
+  XP p = params(a);
+  p.delta = (float*)a->ws;
+  return a->dtype == DH_BF16 ? XATTN_HD(bwd_hd, bf16_t, p, a, (hipStream_t)stream) : XATTN_HD(bwd_hd, float, p, a, (hipStream_t)stream);
+}

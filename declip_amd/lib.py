@@ -5,7 +5,7 @@ fails, a DeclipHipError is raised (never a silent PyTorch/CPU path).
 """
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int64, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int64, c_void_p
 
 import torch
 
@@ -59,6 +59,21 @@ class BlockArgs(Structure):
                 ("ln_nb1", c_int), ("ln_nb2", c_int), ("dw_first_touch", c_int)]
 
 
+class XattnArgs(Structure):
+    """dh_xattn_args (include/declip_hip.h)"""
+    _fields_ = ([(n, c_int) for n in ("dtype", "batch", "heads", "kv_heads", "hd", "rows_q", "rows_kv", "max_q", "max_kv")] + [("scale", c_float)]
+                + [f for n, l in (("q", "ldq"), ("k", "ldk"), ("v", "ldv"), ("out", "ldo")) for f in ((n, c_void_p), (l, c_int64))] + [("lse", c_void_p)]
+                + [f for n, l in (("dout", "lddo"), ("dq", "lddq"), ("dk", "lddk"), ("dv", "lddv")) for f in ((n, c_void_p), (l, c_int64))]
+                + [(n, c_void_p) for n in ("cu_q", "cu_kv", "kv_len", "key_mask", "ws")] + [("ws_bytes", c_int64)])
+
+
+class JoinNormArgs(Structure):
+    """dh_join_norm_args (include/declip_hip.h)"""
+    _fields_ = ([(n, c_int) for n in ("dtype", "rows", "d", "rms", "gate_rows", "gate_channel", "gate_tanh")] + [("alpha", c_float), ("eps", c_float)]
+                + [(n, c_void_p) for n in ("x", "y", "post_w", "post_b", "gate", "scale", "pre_w", "pre_b", "x_out", "n", "stats", "dx_out", "dn", "dx", "dy",
+                                           "d_post_w", "d_post_b", "d_gate", "d_scale", "d_pre_w", "d_pre_b", "ws")] + [("ws_bytes", c_int64)])
+
+
 _P = c_void_p
 _PROTOS = {
     "dh_bpe_create": (c_void_p, [c_char_p, c_int64, c_int]),
@@ -94,6 +109,13 @@ _PROTOS = {
     "dh_attn_bucketed_bwd": (c_int, [c_int, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P]),
     "dh_attn_pooled_fwd": (c_int, [c_int, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P]),
     "dh_attn_pooled_bwd": (c_int, [c_int, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P]),
+    "dh_xattn_ws_bytes": (c_int64, [POINTER(XattnArgs), c_int]),
+    "dh_xattn_fwd": (c_int, [POINTER(XattnArgs), _P]),
+    "dh_xattn_bwd": (c_int, [POINTER(XattnArgs), _P]),
+    "dh_rope_axes": (c_int, [c_int, _P, c_int64, _P, c_int64, c_int, c_int, c_int, _P, c_int, c_int, POINTER(c_int), POINTER(c_double), c_int, c_int, c_int, c_int, _P]),
+    "dh_join_norm_fwd": (c_int, [POINTER(JoinNormArgs), _P]),
+    "dh_join_norm_bwd_ws_bytes": (c_int64, [POINTER(JoinNormArgs)]),
+    "dh_join_norm_bwd": (c_int, [POINTER(JoinNormArgs), _P]),
     "dh_text_embed_fwd": (c_int, [c_int, _P, _P, _P, _P, c_int, c_int, c_int, _P]),
     "dh_text_embed_bwd": (c_int, [c_int, _P, _P, _P, _P, c_int, c_int, c_int, POINTER(c_int64), c_int, _P]),
     "dh_embed_table_grad_ws_bytes": (c_int64, [c_int, c_int]),

@@ -3,6 +3,8 @@
 These only validate shapes, allocate outputs with torch (memory plumbing) and enqueue the
 HIP kernel on torch's current stream.  No arithmetic happens in Python/PyTorch here.
 """
+import collections
+import contextlib
 import ctypes
 
 import torch
@@ -865,3 +867,184 @@ def attnpool_tokens_bwd(dtok, dpos, b, HW):
     dx = torch.empty(b * HW, C, device=dtok.device, dtype=dtok.dtype)
     check(L.load().dh_attnpool_tokens_bwd(dt(dtok), ptr(dtok), ptr(dx), ptr(dpos), b, HW, C, stream()), "dh_attnpool_tokens_bwd")
     return dx
+
+
+# ---------------------------------------------------------------------------------------------
+# operators between the towers (csrc/xattn.hip, rope.hip, join_norm.hip); their autograd functions: declip_amd/fusion.py
+# ---------------------------------------------------------------------------------------------
+def _on_device_of(t, *others):
+    """All tensors of a call lie on one device; the launch goes to that device and its current stream, whatever the current device is."""
+    for o in others:
+        _req(o is None or o.device == t.device, "tensors on different devices (%s, %s)" % (t.device, None if o is None else o.device))
+    if t.is_cuda and t.device.index != torch.cuda.current_device():
+        return torch.cuda.device(t.device)
+    return contextlib.nullcontext()
+
+
+def _rows2d(t, name, width=None):
+    """a [rows, width] tensor with contiguous columns -> its row stride in elements"""
+    _req(t.dim() == 2 and (width is None or t.shape[1] == width) and (t.shape[1] == 1 or t.stride(1) == 1),
+         "%s: [rows, %s] with contiguous columns" % (name, "width" if width is None else width))
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _table(t, name, n):
+    _req(t is None or (t.dtype == torch.int32 and t.numel() == n and t.is_contiguous()), "%s: contiguous int32 [%d]" % (name, n))
+    return t
+
+
+def _xattn_args(q, k, v, heads, kv_heads, batch, cu_q, cu_kv, kv_len, key_mask, scale, max_q, max_kv):
+    heads = int(heads)
+    kv_heads = heads if kv_heads is None else int(kv_heads)
+    _req(q.dim() == 2 and heads > 0 and kv_heads > 0 and heads % kv_heads == 0 and q.shape[1] % heads == 0, "q [rows, heads * hd], heads a multiple of kv_heads")
+    hd = q.shape[1] // heads
+    for n in (cu_q, cu_kv):
+        if n is not None:
+            _req(n.numel() >= 2 and (batch is None or batch == n.numel() - 1), "cu_q / cu_kv [batch + 1]")
+            batch = n.numel() - 1
+    _req(batch is not None and batch > 0, "batch: the number of sequences (or a cu_q / cu_kv table)")
+    _req(q.dtype == k.dtype == v.dtype, "q, k, v of one dtype")
+    _req(k.shape == v.shape, "k and v of one shape")
+    a = L.XattnArgs()
+    a.dtype, a.batch, a.heads, a.kv_heads, a.hd = dt(q), int(batch), heads, kv_heads, hd
+    a.rows_q, a.rows_kv, a.max_q, a.max_kv = q.shape[0], k.shape[0], int(max_q or 0), int(max_kv or 0)
+    a.scale = float(scale) if scale is not None else hd ** -0.5
+    a.ldq, a.ldk, a.ldv = _rows2d(q, "q"), _rows2d(k, "k", kv_heads * hd), _rows2d(v, "v", kv_heads * hd)
+    a.q, a.k, a.v = ptr(q), ptr(k), ptr(v)
+    a.cu_q, a.cu_kv = ptr(_table(cu_q, "cu_q", a.batch + 1)), ptr(_table(cu_kv, "cu_kv", a.batch + 1))
+    a.kv_len = ptr(_table(kv_len, "kv_len", a.batch))
+    if key_mask is not None:
+        _req(key_mask.dtype in (torch.bool, torch.uint8) and key_mask.numel() == a.rows_kv and key_mask.is_contiguous(), "key_mask: contiguous bool / uint8, one per key row")
+        a.key_mask = ptr(key_mask)
+    return a
+
+
+def xattn_fwd(q, k, v, heads, *, kv_heads=None, batch=None, cu_q=None, cu_kv=None, kv_len=None, key_mask=None, scale=None, max_q=None, max_kv=None):
+    """Cross attention to an encoder's states of another length (dh_xattn_fwd): q [rows_q, heads*hd], k / v [rows_kv, kv_heads*hd] (rows may be strided:
+    the halves of one projection) -> (out [rows_q, heads*hd], lse [heads, rows_q] fp32).
+    Sequence i: query rows cu_q[i] .. cu_q[i+1], key rows cu_kv[i] .. cu_kv[i+1] (int32, on the device; None: `batch` equal parts), of which the first
+    kv_len[i] (None: all) with key_mask != 0 (None: all) are keys.  No key: out = 0, lse = -inf.  hd: a multiple of 8 up to 128; max_q / max_kv: the
+    longest sequence if the caller knows it (grid layout only).  scale: hd ** -0.5."""
+    with _on_device_of(q, k, v, cu_q, cu_kv, kv_len, key_mask):
+        a = _xattn_args(q, k, v, heads, kv_heads, batch, cu_q, cu_kv, kv_len, key_mask, scale, max_q, max_kv)
+        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        lse = torch.empty(a.heads, a.rows_q, device=q.device, dtype=torch.float32)
+        a.out, a.ldo, a.lse = ptr(out), out.shape[1], ptr(lse)
+        lib = L.load()
+        need = lib.dh_xattn_ws_bytes(ctypes.byref(a), 0)
+        if need > 0:
+            ws = torch.empty(need // 4, device=q.device, dtype=torch.float32)
+            a.ws, a.ws_bytes = ptr(ws), need
+        check(lib.dh_xattn_fwd(ctypes.byref(a), stream()), "dh_xattn_fwd")
+    return out, lse
+
+
+def xattn_bwd(q, k, v, out, dout, lse, heads, *, kv_heads=None, batch=None, cu_q=None, cu_kv=None, kv_len=None, key_mask=None, scale=None, max_q=None, max_kv=None):
+    """Gradients of xattn_fwd (same geometry arguments; out, lse: its results) -> (dq, dk, dv), contiguous."""
+    with _on_device_of(q, k, v, out, dout, lse, cu_q, cu_kv, kv_len, key_mask):
+        a = _xattn_args(q, k, v, heads, kv_heads, batch, cu_q, cu_kv, kv_len, key_mask, scale, max_q, max_kv)
+        _req(out.shape == q.shape == dout.shape and out.dtype == q.dtype == dout.dtype, "out and dout like q")
+        _req(lse.shape == (a.heads, a.rows_q) and lse.dtype == torch.float32 and lse.is_contiguous(), "lse: contiguous fp32 [heads, rows_q]")
+        dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
+        a.out, a.ldo, a.lse = ptr(out), _rows2d(out, "out"), ptr(lse)
+        a.dout, a.lddo = ptr(dout), _rows2d(dout, "dout")
+        a.dq, a.lddq, a.dk, a.lddk, a.dv, a.lddv = ptr(dq), q.shape[1], ptr(dk), k.shape[1], ptr(dv), v.shape[1]
+        lib = L.load()
+        need = lib.dh_xattn_ws_bytes(ctypes.byref(a), 1)
+        ws = torch.empty(max(need, 16) // 4, device=q.device, dtype=torch.float32)
+        a.ws, a.ws_bytes = ptr(ws), need
+        check(lib.dh_xattn_bwd(ctypes.byref(a), stream()), "dh_xattn_bwd")
+    return dq, dk, dv
+
+
+def rope_axes(x, pos, heads, sections, theta=10000.0, *, joint=False, interleaved=False, inverse=False, out=None):
+    """Rotary positions with several axes (dh_rope_axes): x [rows, heads*hd] (rows may be strided) -> the rotated rows.  pos [rows or a divisor, axes] int32 or
+    fp32; sections: pairs per axis (2 * sum <= hd, the rest of a head is copied); theta: one base, or one per axis; joint: one frequency ladder shared by
+    the axes; interleaved: pairs of neighbouring columns instead of the two halves; inverse: rotate back (the gradient).  out: x itself (in
+    place) or memory of its own."""
+    heads, sections = int(heads), [int(s) for s in sections]
+    with _on_device_of(x, pos, out):
+        ldx = _rows2d(x, "x")
+        _req(heads > 0 and x.shape[1] % heads == 0 and x.shape[1] > 0, "x [rows, heads * hd]")
+        _req(pos.dim() == 2 and pos.shape[1] == len(sections) and pos.is_contiguous() and pos.dtype in (torch.int32, torch.float32), "pos: contiguous int32 / fp32 [rows, axes]")
+        if out is None:
+            out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        else:
+            same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
+            _req(out.shape == x.shape and out.dtype == x.dtype and (same or out.untyped_storage().data_ptr() != x.untyped_storage().data_ptr()),
+                 "out: like x, x itself or memory of its own")
+        ths = [float(t) for t in theta] if isinstance(theta, (tuple, list)) else [float(theta)] * len(sections)
+        _req(len(ths) == len(sections), "theta: one, or one per axis")
+        n = len(sections)
+        check(L.load().dh_rope_axes(dt(x), ptr(x), ldx, ptr(out), _rows2d(out, "out"), x.shape[0], heads, x.shape[1] // heads, ptr(pos), int(pos.dtype == torch.float32),
+                                    pos.shape[0], (ctypes.c_int * n)(*sections), (ctypes.c_double * n)(*ths), n, int(joint), int(interleaved), int(inverse),
+                                    stream()), "dh_rope_axes")
+    return out
+
+
+JoinNormGrads = collections.namedtuple("JoinNormGrads", "post_w post_b gate scale pre_w pre_b")
+
+
+def _join_args(x, y, post, gate, scale, pre, alpha, eps, rms, gate_tanh):
+    _req(x.dim() == 2 and x.shape == y.shape and x.dtype == y.dtype, "x and y [rows, d] of one dtype")
+    rows, d = x.shape
+    a = L.JoinNormArgs()
+    a.dtype, a.rows, a.d, a.rms, a.gate_tanh, a.alpha, a.eps = dt(x), rows, d, int(rms), int(gate_tanh), float(alpha), float(eps)
+    a.x, a.y = ptr(_contig(x, "x")), ptr(_contig(y, "y"))
+
+    def vec(t, name):
+        _req(t is None or (t.dtype == torch.float32 and t.numel() == d and t.is_contiguous()), "%s: contiguous fp32 [d]" % name)
+        return ptr(t)
+
+    if post is not None:
+        a.post_w, a.post_b = vec(post[0], "post weight"), vec(post[1], "post bias")
+    if pre is not None:
+        a.pre_w, a.pre_b = vec(pre[0], "pre weight"), vec(pre[1], "pre bias")
+    a.scale = vec(scale, "scale")
+    if gate is not None:
+        _req(gate.dtype == torch.float32 and gate.is_contiguous() and gate.dim() <= 2 and (gate.dim() < 2 or gate.shape[1] == d), "gate: contiguous fp32 [groups] or [groups, d]")
+        a.gate_rows, a.gate_channel = (gate.shape[0] if gate.dim() else 1), int(gate.dim() == 2)
+        _req(a.gate_rows > 0 and rows % a.gate_rows == 0, "gate: %d groups of %d rows" % (a.gate_rows, rows))
+        a.gate = ptr(gate)
+    return a
+
+
+def _join_tensors(post, gate, scale, pre):
+    return [*(post or (None, None)), gate, scale, *(pre or (None, None))]
+
+
+def join_norm_fwd(x, y, *, post=None, gate=None, scale=None, pre=None, alpha=1.0, eps=1e-5, rms=False, gate_tanh=False):
+    """A block's boundary in one pass (dh_join_norm_fwd): x_out = alpha x + scale * g * N_post(y), n = N_pre(x_out) -> (x_out, n or None, stats).
+    x (residual stream), y (the block's output) [rows, d]; post / pre: (weight, bias or None) fp32 or None (no such norm); gate: fp32 [groups] or [groups, d],
+    one value or vector per rows / groups consecutive rows (gate_tanh: tanh of it); scale: fp32 [d]; rms: RMS norms instead of LayerNorms."""
+    with _on_device_of(x, y, *_join_tensors(post, gate, scale, pre)):
+        a = _join_args(x, y, post, gate, scale, pre, alpha, eps, rms, gate_tanh)
+        x_out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        n = torch.empty(x.shape, device=x.device, dtype=x.dtype) if pre is not None else None
+        stats = torch.empty(4, a.rows, device=x.device, dtype=torch.float32)
+        a.x_out, a.n, a.stats = ptr(x_out), ptr(n), ptr(stats)
+        check(L.load().dh_join_norm_fwd(ctypes.byref(a), stream()), "dh_join_norm_fwd")
+    return x_out, n, stats
+
+
+def join_norm_bwd(x, y, dx_out, dn, stats, *, post=None, gate=None, scale=None, pre=None, alpha=1.0, eps=1e-5, rms=False, gate_tanh=False):
+    """Gradients of join_norm_fwd (same arguments, stats: its third result; dx_out or dn may be None) -> (dx, dy, JoinNormGrads); parameter gradients
+    are new fp32 tensors of their parameter's shape, None where there is no parameter."""
+    params = _join_tensors(post, gate, scale, pre)
+    with _on_device_of(x, y, dx_out, dn, stats, *params):
+        a = _join_args(x, y, post, gate, scale, pre, alpha, eps, rms, gate_tanh)
+        for t, name in ((dx_out, "dx_out"), (dn, "dn")):
+            _req(t is None or (t.shape == x.shape and t.dtype == x.dtype and t.is_contiguous()), "%s: like x, contiguous" % name)
+        _req(stats.shape == (4, a.rows) and stats.dtype == torch.float32 and stats.is_contiguous(), "stats: the forward's")
+        dx, dy = torch.empty(x.shape, device=x.device, dtype=x.dtype), torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        if a.rows == 0:
+            return dx, dy, JoinNormGrads(*(None if t is None else torch.zeros_like(t) for t in params))
+        grads = JoinNormGrads(*(None if t is None else torch.empty_like(t) for t in params))
+        a.dx_out, a.dn, a.stats, a.dx, a.dy = ptr(dx_out), ptr(dn), ptr(stats), ptr(dx), ptr(dy)
+        a.d_post_w, a.d_post_b, a.d_gate, a.d_scale, a.d_pre_w, a.d_pre_b = (ptr(t) for t in grads)
+        lib = L.load()
+        need = lib.dh_join_norm_bwd_ws_bytes(ctypes.byref(a))
+        ws = torch.empty(max(need, 16) // 4, device=x.device, dtype=torch.float32)
+        a.ws, a.ws_bytes = ptr(ws), need
+        check(lib.dh_join_norm_bwd(ctypes.byref(a), stream()), "dh_join_norm_bwd")
+    return dx, dy, grads

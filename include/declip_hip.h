@@ -188,6 +188,80 @@ int dh_attn_pooled_fwd(int dtype, const void* q, const void* kv, void* out, floa
 int dh_attn_pooled_bwd(int dtype, const void* q, const void* kv, const void* dout, const float* lse, void* dq, void* dkv,
                        const int* row0, const int* nkeys, int b, int heads, int hd, int Lmax, int total_rows, dh_stream_t stream);
 
+/* ---------------------------------------------------------------- cross attention -------
+ * Attention of one batch's queries over an encoder's states of ANOTHER length (a caption decoder or fusion tower over the image tower's
+ * tokens; the reference declares such a branch, return_caption of model/declip.py:166-167, and never builds it):
+ *   s = scale q k^T over the valid keys, p = softmax(s), out = p v, lse = log sum exp s
+ * Layout: token-major rows, head-major columns.  q / out / dout / dq [rows_q][heads*hd], k / v / dk / dv [rows_kv][kv_heads*hd], each with its own
+ * row stride in elements (k and v may be the halves of one [rows][2*kv_heads*hd] projection), 16-byte aligned rows; lse [heads][rows_q] fp32.
+ *   heads % kv_heads == 0: query head h reads kv head h / (heads / kv_heads) and dk / dv are summed over it.  hd: a multiple of 8 up to 128.
+ *   Sequence i owns query rows cu_q[i] .. cu_q[i+1] and key rows cu_kv[i] .. cu_kv[i+1] (int32 [batch + 1], device memory, ascending); a NULL
+ *   table means rows / batch rows each.  kv_len (int32 [batch], or NULL): only the first kv_len[i] of them are keys.  key_mask (1 byte per key
+ *   row, or NULL): 0 = not a key.  What k / v hold in rows that are no keys is never used, NaN included; their dk / dv are 0.
+ *   A query without any key: out = 0, lse = -inf, no gradient.  Rows outside [cu[0], cu[batch]) are written as zeros (lse -inf).
+ *   max_q / max_kv: longest query / key row count of a sequence as far as the caller knows it (0: unknown), used to lay out the grid only --
+ *   longer sequences are computed whole.  Table entries are clamped to the row counts, so no table makes a kernel leave its buffers.
+ *   scale > 0.  bf16: P and dS are rounded to bf16 as MFMA operands; statistics, sums and accumulators fp32.  No atomics: the same bits on every run.
+ * fwd reads q k v, writes out lse; bwd reads q k v out dout lse, writes dq dk dv.  ws: dh_xattn_ws_bytes(args, backward) bytes of scratch, 16-byte
+ * aligned, not shared with anything that may run at the same time. */
+typedef struct {
+  int dtype, batch, heads, kv_heads, hd;
+  int rows_q, rows_kv, max_q, max_kv;
+  float scale;
+  const void* q; int64_t ldq;
+  const void* k; int64_t ldk;
+  const void* v; int64_t ldv;
+  void* out; int64_t ldo;                 /* fwd: output; bwd: input */
+  float* lse;                             /* fwd: output; bwd: input */
+  const void* dout; int64_t lddo;
+  void* dq; int64_t lddq;
+  void* dk; int64_t lddk;
+  void* dv; int64_t lddv;
+  const int* cu_q; const int* cu_kv; const int* kv_len; const uint8_t* key_mask;
+  void* ws; int64_t ws_bytes;
+} dh_xattn_args;
+int64_t dh_xattn_ws_bytes(const dh_xattn_args* args, int backward);   /* -1: the arguments are refused */
+int dh_xattn_fwd(const dh_xattn_args* args, dh_stream_t stream);
+int dh_xattn_bwd(const dh_xattn_args* args, dh_stream_t stream);
+
+/* ---------------------------------------------------------------- rotary positions ------
+ * Rotary positions with several axes (time, height, width of image / video tokens) on `heads` heads of hd columns each; beside the learned
+ * tables of image_encoder/visual_transformer.py:20-22 and text_encoder/text_transformer.py:99.  x [rows][>= heads*hd] (row stride ldx; e.g. the q
+ * and k columns of a fused projection as 2*heads heads), y likewise, y == x allowed (in place), otherwise disjoint.
+ * Axis a turns sections[a] pairs, in the order of the axes; P = their sum, 2 P <= hd, P <= 128; columns behind 2 P of a head are copied.
+ *   pair i = columns (i, P + i), interleaved: (2 i, 2 i + 1) of a head
+ *   angle  = pos[row % pos_rows][axis] * theta[axis] ^ (-j / sections[axis]), j = the pair's place in its axis (joint: theta ^ (-i / P))
+ *   (a, b) -> (a cos - b sin, a sin + b cos); inverse = 1 turns by -angle: the gradient of the rotation
+ * pos [pos_rows][axes] int32, or fp32 (pos_float = 1); rows % pos_rows == 0 (a batch of equal grids shares one table).  Angles are formed in 64 bits. */
+int dh_rope_axes(int dtype, const void* x, int64_t ldx, void* y, int64_t ldy, int rows, int heads, int hd, const void* pos, int pos_float,
+                 int pos_rows, const int* sections, const double* theta, int axes, int joint, int interleaved, int inverse, dh_stream_t stream);
+
+/* ---------------------------------------------------------------- block boundary --------
+ * The norm behind a block, its gate and residual scale, the residual sum and the norm in front of the next block in one pass (the residual
+ * boundary of base_transformer.py:50-53, with the terms deeper and adapted towers add):
+ *   p = N_post(y) (post_w NULL: y);   x_out = alpha x + scale[c] g p (scale NULL: 1);   n = N_pre(x_out) (pre_w NULL: no n)
+ *   N: LayerNorm (z - mean) rstd w + b (b may be NULL), or RMS norm z rstd w (rms = 1); fp32 parameters [d]
+ *   g: 1 (gate NULL) or gate (gate_tanh: tanh(gate)), fp32, one value per rows / gate_rows consecutive rows ([gate_rows]) or one
+ *   vector ([gate_rows][d], gate_channel = 1)
+ * x, y, x_out, n, dx_out, dn, dx, dy [rows][d] contiguous, d <= 8192; 16-byte accesses where d % 8 == 0 and the addresses allow it.
+ * stats [4][rows] fp32: mean / rstd of both norms, written by fwd, read by bwd.  n is computed from x_out before its rounding to dtype.
+ * bwd: dx_out and dn are the gradients of the two outputs (one may be NULL); parameter gradients are WRITTEN (not accumulated), fp32, NULL =
+ * not wanted; ws: dh_join_norm_bwd_ws_bytes(args).  No atomics: the same bits on every run. */
+typedef struct {
+  int dtype, rows, d;
+  int rms, gate_rows, gate_channel, gate_tanh;
+  float alpha, eps;
+  const void* x; const void* y;
+  const float* post_w; const float* post_b; const float* gate; const float* scale; const float* pre_w; const float* pre_b;
+  void* x_out; void* n; float* stats;
+  const void* dx_out; const void* dn; void* dx; void* dy;
+  float* d_post_w; float* d_post_b; float* d_gate; float* d_scale; float* d_pre_w; float* d_pre_b;
+  void* ws; int64_t ws_bytes;
+} dh_join_norm_args;
+int dh_join_norm_fwd(const dh_join_norm_args* args, dh_stream_t stream);
+int64_t dh_join_norm_bwd_ws_bytes(const dh_join_norm_args* args);     /* -1: the arguments are refused */
+int dh_join_norm_bwd(const dh_join_norm_args* args, dh_stream_t stream);
+
 /* ---------------------------------------------------------------- one transformer block per call
  * ResidualAttentionBlock (base_transformer.py:29-53): x_mid = x + out_proj(attn(in_proj(ln_1(x)))), x_out = x_mid +
  * c_proj(quick_gelu(c_fc(ln_2(x_mid)))), and its backward -- enqueued by ONE call: 9 launches forward, 13 backward (the four

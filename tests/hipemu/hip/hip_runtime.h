@@ -47,6 +47,10 @@ static inline float __int_as_float(int u) { float f; memcpy(&f, &u, 4); return f
 static inline int __float_as_int(float f) { int u; memcpy(&u, &f, 4); return u; }
 #define __expf expf
 #define __logf logf
+#define __log2f log2f
+#define __builtin_amdgcn_exp2f(x) exp2f(x)
+static inline float cospif(float x) { return (float)cos(M_PI * (double)x); }
+static inline float sinpif(float x) { return (float)sin(M_PI * (double)x); }
 static inline float rsqrtf(float x) { return 1.f / sqrtf(x); }
 static inline float __frcp_rn(float x) { return 1.f / x; }
 static inline float __fdividef(float a, float b) { return a / b; }
