@@ -34,6 +34,7 @@ struct XP {
   const uint8_t* key_mask;
   long ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;
   int rows_q, rows_kv, batch, heads, kv_heads, rep, hd;
+  unsigned magic;     // ceil(2^32 / rep)
   float scale;
   int tiles;          // tiles per (sequence, kv head) in the grid; a block walks t, t + tiles, ... (longer sequences than announced are still whole)
   int nsplit;         // key ranges per tile (forward)
@@ -171,13 +172,21 @@ __device__ __forceinline__ void owned(const int* cu, int batch, int rows, int& f
   last = clampi(cu[batch], first, rows);
 }
 
-// row m of the packed query axis -> offset of its head's elements
+// row m of the packed query axis -> (query, head of the group): the quotient by rep from one high product with magic = ceil(2^32 / rep), which is too
+// large by one at most
+__device__ __forceinline__ void m_split(const XP& p, int m, int& q, int& r) {
+  q = p.rep == 1 ? m : (int)__umulhi((unsigned)m, p.magic);
+  r = m - q * p.rep;
+  if (r < 0) { --q; r += p.rep; }
+}
 __device__ __forceinline__ long m_offset(const XP& p, const Seq& s, int g, int m, long ld) {
-  const int q = p.rep == 1 ? m : m / p.rep, r = m - q * p.rep;
-  return (long)(s.q0 + q) * ld + (long)(g * p.rep + r) * p.hd;
+  int q, r;
+  m_split(p, m, q, r);
+  return (long)(s.q0 + q) * ld + (g * p.rep + r) * p.hd;
 }
 __device__ __forceinline__ long m_stat(const XP& p, const Seq& s, int g, int m) {
-  const int q = p.rep == 1 ? m : m / p.rep, r = m - q * p.rep;
+  int q, r;
+  m_split(p, m, q, r);
   return (long)(g * p.rep + r) * p.rows_q + s.q0 + q;
 }
 
@@ -206,48 +215,127 @@ __device__ __forceinline__ f32x16_t mma_row(const T* tile, int ld, int row0, con
   return c;
 }
 
-// two tiles of ROWS rows on their way from memory to LDS (registers in between)
+// the value of the lane 32 further (the other half of the same row / key column)
+__device__ __forceinline__ float other_half(float v) {
+#ifndef DH_HOST_EMU
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+#else
+  return __shfl_xor(v, 32, 64);
+#endif
+}
+__device__ __forceinline__ float half_max(float v) {
+#ifndef DH_HOST_EMU
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+#else
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+#endif
+}
+
+// Two tiles of ROWS rows on their way from memory to LDS.  fetch() asks for the next tile while the current one is multiplied (16-byte loads, no
+// branch: rows behind the last one read that one again), store() puts it into the other LDS buffer one iteration later.
 template <typename T, int HDP, int ROWS, int NT>
 struct Pair2 {
   static constexpr int EPC = Op<T>::EPC, NCH = HDP / EPC, N = (ROWS * NCH + NT - 1) / NT, LD = HDP + EPC;
+  static constexpr bool RAGGED = ROWS * NCH % NT != 0;      // fewer tasks than threads, or a last round of fewer
   uint4 a[N], b[N];
-  // fa(row) / fb(row): element pointers of a tile row, or nullptr for a row of zeros
+  uint8_t keep[N];
+  // pa / pb: bases; off_a / off_b(row): element offsets of a tile row; last: the last row that exists; mask: a byte per row, or NULL
   template <typename FA, typename FB>
-  __device__ __forceinline__ void fetch(FA fa, FB fb, int hd, int tid) {
+  __device__ __forceinline__ void fetch(const T* pa, const T* pb, FA off_a, FB off_b, int first, int last, const uint8_t* mask, int hd, int tid) {
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      const int task = tid + k * NT, row = task / NCH, c = task % NCH;
-      a[k] = b[k] = make_uint4(0u, 0u, 0u, 0u);
-      if (ROWS * NCH % NT != 0 && task >= ROWS * NCH) continue;
-      if (c * EPC < hd) {
-        const T *pa = fa(row), *pb = fb(row);
-        if (pa) { a[k] = *reinterpret_cast<const uint4*>(pa + c * EPC); b[k] = *reinterpret_cast<const uint4*>(pb + c * EPC); }
-      }
+      if (RAGGED && tid + k * NT >= ROWS * NCH) continue;
+      const int task = tid + k * NT, row = min(first + task / NCH, last), c = (task % NCH) * EPC, col = HDP == hd || c < hd ? c : 0;
+      a[k] = *reinterpret_cast<const uint4*>(pa + off_a(row) + col);
+      b[k] = *reinterpret_cast<const uint4*>(pb + off_b(row) + col);
+      if (mask) keep[k] = mask[row];
     }
   }
-  template <typename FD>
-  __device__ __forceinline__ void store(T* ta, T* tb, FD dead, int tid) {
+  // edge: rows or columns of this tile may have to be zeros (first .. last and mask as fetched)
+  __device__ __forceinline__ void store(T* ta, T* tb, bool edge, int first, int last, bool masked, int hd, int tid) {
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      const int task = tid + k * NT, row = task / NCH, c = task % NCH;
-      if (ROWS * NCH % NT != 0 && task >= ROWS * NCH) continue;
-      if (dead(row)) a[k] = b[k] = make_uint4(0u, 0u, 0u, 0u);
-      *reinterpret_cast<uint4*>(ta + row * LD + c * EPC) = a[k];
-      *reinterpret_cast<uint4*>(tb + row * LD + c * EPC) = b[k];
+      const int task = tid + k * NT, row = task / NCH, c = (task % NCH) * EPC;
+      if (RAGGED && task >= ROWS * NCH) continue;
+      if (edge && (first + row > last || c >= hd || (masked && !keep[k]))) a[k] = b[k] = make_uint4(0u, 0u, 0u, 0u);
+      *reinterpret_cast<uint4*>(ta + row * LD + c) = a[k];
+      *reinterpret_cast<uint4*>(tb + row * LD + c) = b[k];
     }
   }
 };
 
+// The key tiles of a sequence: K and V rows in two LDS buffers, the validity of their keys beside them.
+template <typename T, int HDP, int BN, int NT>
+struct Tiles {
+  static constexpr int LD = HDP + Op<T>::EPC;
+  const T *kb, *vb;
+  const uint8_t* km;
+  T* buf;
+  float* bias;
+  long ldk, ldv;
+  int nk, hd;
+  uint8_t own;                                         // validity of key `tid` of the tile on its way
+  Pair2<T, HDP, BN, NT> st;
+  __device__ __forceinline__ Tiles(const XP& p, const Seq& s, int g, unsigned char* smem) {
+    kb = (const T*)p.k + (long)s.k0 * p.ldk + (long)g * p.hd;
+    vb = (const T*)p.v + (long)s.k0 * p.ldv + (long)g * p.hd;
+    km = p.key_mask ? p.key_mask + s.k0 : nullptr;
+    buf = reinterpret_cast<T*>(smem);
+    bias = reinterpret_cast<float*>(buf + 4 * BN * LD);
+    ldk = p.ldk; ldv = p.ldv; nk = s.nk; hd = p.hd;
+  }
+  __device__ __forceinline__ void fetch(int kt, int tid) {
+    st.fetch(kb, vb, [&](int r) { return (long)r * ldk; }, [&](int r) { return (long)r * ldv; }, kt * BN, nk - 1, km, hd, tid);
+    if (km && tid < BN) own = km[min(kt * BN + tid, nk - 1)];
+  }
+  __device__ __forceinline__ bool edge(int kt) const { return km != nullptr || (kt + 1) * BN > nk; }
+  __device__ __forceinline__ void store(int kt, int tid) {
+    T* b = buf + (kt & 1) * 2 * BN * LD;
+    const bool e = edge(kt);
+    st.store(b, b + BN * LD, e || hd < HDP, kt * BN, nk - 1, km != nullptr, hd, tid);
+    if (e && tid < BN) bias[(kt & 1) * BN + tid] = kt * BN + tid < nk && (!km || own) ? 0.f : -INFINITY;
+  }
+  __device__ __forceinline__ void begin(int lo, int hi, int tid) {
+    if (lo >= hi) return;
+    fetch(lo, tid);
+    store(lo, tid);
+    if (lo + 1 < hi) fetch(lo + 1, tid);
+    __syncthreads();
+  }
+  // tile kt for reading (true: with keys that are none, see bias); the one after it goes to the other buffer, the next but one on its way
+  __device__ __forceinline__ bool next(int kt, int hi, int tid, const T*& ks, const T*& vs, const float*& bi) {
+    if (kt + 1 < hi) {
+      store(kt + 1, tid);
+      if (kt + 2 < hi) fetch(kt + 2, tid);
+    }
+    ks = buf + (kt & 1) * 2 * BN * LD;
+    vs = ks + BN * LD;
+    bi = bias + (kt & 1) * BN;
+    return edge(kt);
+  }
+};
+// scores of keys that are none become -inf (a select, not a sum: such a score may be anything)
+__device__ __forceinline__ void mask_keys(f32x16_t& sc, const float* bias, int h) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float4 bi = *reinterpret_cast<const float4*>(bias + 8 * i + 4 * h);
+    sc[4 * i] = bi.x < 0.f ? -INFINITY : sc[4 * i]; sc[4 * i + 1] = bi.y < 0.f ? -INFINITY : sc[4 * i + 1];
+    sc[4 * i + 2] = bi.z < 0.f ? -INFINITY : sc[4 * i + 2]; sc[4 * i + 3] = bi.w < 0.f ? -INFINITY : sc[4 * i + 3];
+  }
+}
+
 // ------------------------------------------------------------------------------------------ forward
+// waves per SIMD to compile for: two where their registers hold everything (a budget of 256 keeps the accumulators out of the accumulation registers, whose
+// moves cost the rescaled forward 192 instructions a tile), else one
+template <typename T, int HDP, int NW> constexpr int waves_fwd() { return NW == 1 ? (HDP * sizeof(T) <= 128 ? 2 : 1) : (HDP * sizeof(T) <= 384 ? 2 : 1); }
 template <typename T, int HDP, int NW, int BN, bool SPLIT>
-__global__ __launch_bounds__(64 * NW) void xattn_fwd_kernel(XP p) {
+__global__ __launch_bounds__(64 * NW, (waves_fwd<T, HDP, NW>())) void xattn_fwd_kernel(XP p) {
   constexpr int EPC = Op<T>::EPC, LD = HDP + EPC, KS = HDP / (2 * EPC), DB = HDP / 32, NB = BN / 32, BM = 32 * NW, NT = 64 * NW;
   DH_DYN_LDS_A16(unsigned char, smem);
-  T* Ks = reinterpret_cast<T*>(smem);
-  T* Vs = Ks + BN * LD;
-  float* bias = reinterpret_cast<float*>(Vs + BN * LD);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-  const T *q = (const T*)p.q, *kp = (const T*)p.k, *vp = (const T*)p.v;
+  const T* q = (const T*)p.q;
   if ((int)blockIdx.x >= p.main_blocks) {
     int first, last;
     owned(p.cu_q, p.batch, p.rows_q, first, last);
@@ -272,10 +360,6 @@ __global__ __launch_bounds__(64 * NW) void xattn_fwd_kernel(XP p) {
     hi = min(lo + per, nt);
   }
   const float c = p.scale * kLog2e;
-  const uint8_t* km = p.key_mask ? p.key_mask + s.k0 : nullptr;
-  const T* kb_ = kp + (long)s.k0 * p.ldk + (long)w.g * p.hd;
-  const T* vb_ = vp + (long)s.k0 * p.ldv + (long)w.g * p.hd;
-
   for (int t = w.t; (long)t * BM < M; t += p.tiles) {
     const int m = t * BM + wave * 32 + (lane & 31);
     const bool live = m < M, wave_live = t * BM + wave * 32 < M;
@@ -287,69 +371,58 @@ __global__ __launch_bounds__(64 * NW) void xattn_fwd_kernel(XP p) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
     float mrun = -INFINITY, l = 0.f;
-    Pair2<T, HDP, BN, NT> st;
-    auto fetch = [&](int kt) {
-      st.fetch([&](int r) -> const T* { const int key = kt * BN + r; return key < s.nk ? kb_ + (long)key * p.ldk : nullptr; },
-               [&](int r) -> const T* { return vb_ + (long)(kt * BN + r) * p.ldv; }, p.hd, tid);
-    };
-    if (lo < hi) fetch(lo);
+    Tiles<T, HDP, BN, NT> kt_(p, s, w.g, smem);
+    kt_.begin(lo, hi, tid);
     for (int kt = lo; kt < hi; ++kt) {
-      __syncthreads();                               // the tile before is read
-      st.store(Ks, Vs, [&](int r) { const int key = kt * BN + r; return km != nullptr && key < s.nk && !km[key]; }, tid);
-      const bool masked = km != nullptr || (kt + 1) * BN > s.nk;
-      if (masked)
-        for (int r = tid; r < BN; r += NT) {
-          const int key = kt * BN + r;
-          bias[r] = key < s.nk && (!km || km[key]) ? 0.f : -INFINITY;
-        }
-      __syncthreads();
-      if (kt + 1 < hi) fetch(kt + 1);
-      if (!wave_live) continue;
-      f32x16_t sc[NB];
+      const T *Ks, *Vs;
+      const float* bias;
+      const bool masked = kt_.next(kt, hi, tid, Ks, Vs, bias);
+      if (wave_live) {
+        f32x16_t sc[NB];
 #pragma unroll
-      for (int b = 0; b < NB; ++b) sc[b] = mma_row<T, HDP>(Ks, LD, b * 32, qf, lane);
-      if (masked) {
+        for (int b = 0; b < NB; ++b) sc[b] = mma_row<T, HDP>(Ks, LD, b * 32, qf, lane);
+        if (masked) {
+#pragma unroll
+          for (int b = 0; b < NB; ++b) mask_keys(sc[b], bias + b * 32, h);
+        }
+        float mx = sc[0][0];
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float4 bi = *reinterpret_cast<const float4*>(bias + b * 32 + 8 * i + 4 * h);
-            // (a select, not a sum: a masked score may be anything)
-            sc[b][4 * i] = bi.x < 0.f ? -INFINITY : sc[b][4 * i]; sc[b][4 * i + 1] = bi.y < 0.f ? -INFINITY : sc[b][4 * i + 1];
-            sc[b][4 * i + 2] = bi.z < 0.f ? -INFINITY : sc[b][4 * i + 2]; sc[b][4 * i + 3] = bi.w < 0.f ? -INFINITY : sc[b][4 * i + 3];
-          }
-      }
-      float mx = sc[0][0];
+          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[b][i]);
+        mx = half_max(mx) * c;
+        // the running maximum follows only when a score passes it by 2^8: p stays below 2^8, and most tiles leave the sums as they are
+        const bool up = mx > mrun + 8.f;
+        if (__any(up)) {
+          const float mnew = up ? mx : mrun, alpha = mrun == -INFINITY ? 0.f : exp2_fast(mrun - mnew);
+          mrun = mnew;
+          l *= alpha;
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
+          for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[b][i]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      const float mnew = fmaxf(mrun, mx * c), ms = mnew == -INFINITY ? 0.f : mnew;
-      const float alpha = exp2_fast(mrun - ms);
-      mrun = mnew;
-      float sum = 0.f;
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float e = exp2_fast(fmaf(sc[b][i], c, -ms));
-          sc[b][i] = e;
-          sum += e;
+            for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
         }
-      l = fmaf(l, alpha, sum);                       // this half-wave's keys; joined behind the loop
+        const float ms = mrun == -INFINITY ? 0.f : mrun;
+        float sum = 0.f;
 #pragma unroll
-      for (int d = 0; d < DB; ++d)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+          for (int i = 0; i < 16; ++i) {
+            const float e = exp2_fast(fmaf(sc[b][i], c, -ms));
+            sc[b][i] = e;
+            sum += e;
+          }
+        l += sum;                                      // this half-wave's keys; joined behind the loop
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const typename Op<T>::PF pf = Op<T>::pack(sc[b]);
+        for (int b = 0; b < NB; ++b) {
+          const typename Op<T>::PF pf = Op<T>::pack(sc[b]);
 #pragma unroll
-        for (int d = 0; d < DB; ++d) Op<T>::mma_t(o[d], Vs, LD, b * 32, d * 32, pf, lane);
+          for (int d = 0; d < DB; ++d) Op<T>::mma_t(o[d], Vs, LD, b * 32, d * 32, pf, lane);
+        }
       }
+      __syncthreads();                                 // this buffer is read, the other one written
     }
-    l += __shfl_xor(l, 32, 64);
+    l += other_half(l);
     if (live) {
       const long stat = m_stat(p, s, w.g, m);
       if (SPLIT) {
@@ -381,45 +454,43 @@ __global__ __launch_bounds__(64 * NW) void xattn_fwd_kernel(XP p) {
   }
 }
 
-// joins the key ranges of one (query row, head): o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, ranges in ascending order
+// joins the key ranges of one (query row, head): o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, ranges in ascending order.  A wave per pair: its lanes
+// read the ranges' (m, l) at once, and a lane's columns of the partial sums are independent loads.
 template <typename T>
 __global__ __launch_bounds__(256) void xattn_join_kernel(XP p) {
   int first = 0, last = p.rows_q;
   if (p.cu_q) owned(p.cu_q, p.batch, p.rows_q, first, last);
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, c0 = 2 * lane;
   const long n = (long)(last - first) * p.heads, stride = (long)p.heads * p.rows_q;
   for (long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += (long)gridDim.x * 4) {
     const int row = first + (int)(i / p.heads), head = (int)(i % p.heads);
     const long stat = (long)head * p.rows_q + row;
-    float m = -INFINITY;
-    for (int s = 0; s < p.nsplit; ++s) m = fmaxf(m, p.part_ml[2 * (s * stride + stat)]);
-    const float ms = m == -INFINITY ? 0.f : m;
-    float l = 0.f, a0 = 0.f, a1 = 0.f;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (lane < p.nsplit) ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * (lane * stride + stat));
+    const float m = wave_max(ml.x), f = ml.y == 0.f ? 0.f : exp2_fast(ml.x - m), l = wave_sum(f * ml.y);
+    float2 acc = make_float2(0.f, 0.f);
+    const float* part = p.part_o + stat * p.hd + c0;
+#pragma unroll 4
     for (int s = 0; s < p.nsplit; ++s) {
-      const long part = s * stride + stat;
-      const float ml = p.part_ml[2 * part + 1];
-      if (ml == 0.f) continue;                       // an empty range wrote no sums
-      const float f = exp2_fast(p.part_ml[2 * part] - ms);
-      l = fmaf(f, ml, l);
-      if (lane < p.hd) a0 = fmaf(f, p.part_o[part * p.hd + lane], a0);
-      if (lane + 64 < p.hd) a1 = fmaf(f, p.part_o[part * p.hd + lane + 64], a1);
+      const float fs = __shfl(f, s, 64);
+      if (fs != 0.f && c0 < p.hd) {                  // (an empty range wrote no sums)
+        const float2 v = *reinterpret_cast<const float2*>(part + s * stride * p.hd);
+        acc.x = fmaf(fs, v.x, acc.x);
+        acc.y = fmaf(fs, v.y, acc.y);
+      }
     }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    T* o = (T*)p.out + (long)row * p.ldo + (long)head * p.hd;
-    if (lane < p.hd) st<T>(o + lane, a0 * inv);
-    if (lane + 64 < p.hd) st<T>(o + lane + 64, a1 * inv);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* o = (T*)p.out + (long)row * p.ldo + (long)head * p.hd + c0;
+    if (c0 < p.hd) { st<T>(o, acc.x * inv); st<T>(o + 1, acc.y * inv); }
     if (lane == 0) p.lse[stat] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
   }
 }
 
 // ------------------------------------------------------------------------------------------ backward: dq (and D)
 template <typename T, int HDP, int NW, int BN>
-__global__ __launch_bounds__(64 * NW) void xattn_dq_kernel(XP p) {
+__global__ __launch_bounds__(64 * NW, NW == 8 || HDP <= 64 ? 2 : 1) void xattn_dq_kernel(XP p) {
   constexpr int EPC = Op<T>::EPC, LD = HDP + EPC, KS = HDP / (2 * EPC), DB = HDP / 32, NB = BN / 32, BM = 32 * NW, NT = 64 * NW;
   DH_DYN_LDS_A16(unsigned char, smem);
-  T* Ks = reinterpret_cast<T*>(smem);
-  T* Vs = Ks + BN * LD;
-  float* bias = reinterpret_cast<float*>(Vs + BN * LD);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
   if ((int)blockIdx.x >= p.main_blocks) {
     int first, last;
@@ -432,9 +503,6 @@ __global__ __launch_bounds__(64 * NW) void xattn_dq_kernel(XP p) {
   const Seq s = seq_of(p, w.b);
   const int M = s.nq * p.rep, nt = (s.nk + BN - 1) / BN;
   const float c = p.scale * kLog2e;
-  const uint8_t* km = p.key_mask ? p.key_mask + s.k0 : nullptr;
-  const T* kb_ = (const T*)p.k + (long)s.k0 * p.ldk + (long)w.g * p.hd;
-  const T* vb_ = (const T*)p.v + (long)s.k0 * p.ldv + (long)w.g * p.hd;
   for (int t = w.t; (long)t * BM < M; t += p.tiles) {
     const int m = t * BM + wave * 32 + (lane & 31);
     const bool live = m < M, wave_live = t * BM + wave * 32 < M;
@@ -452,69 +520,53 @@ __global__ __launch_bounds__(64 * NW) void xattn_dq_kernel(XP p) {
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) D += Op<T>::dot(df[ks], of[ks]);
     }
-    D += __shfl_xor(D, 32, 64);
+    D += other_half(D);
     if (live && h == 0) p.delta[stat] = D;
     f32x16_t dq[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) dq[d][i] = 0.f;
-    Pair2<T, HDP, BN, NT> st;
-    auto fetch = [&](int kt) {
-      st.fetch([&](int r) -> const T* { const int key = kt * BN + r; return key < s.nk ? kb_ + (long)key * p.ldk : nullptr; },
-               [&](int r) -> const T* { return vb_ + (long)(kt * BN + r) * p.ldv; }, p.hd, tid);
-    };
-    if (nt > 0) fetch(0);
+    Tiles<T, HDP, BN, NT> kt_(p, s, w.g, smem);
+    kt_.begin(0, nt, tid);
     for (int kt = 0; kt < nt; ++kt) {
-      __syncthreads();
-      st.store(Ks, Vs, [&](int r) { const int key = kt * BN + r; return km != nullptr && key < s.nk && !km[key]; }, tid);
-      const bool masked = km != nullptr || (kt + 1) * BN > s.nk;
-      if (masked)
-        for (int r = tid; r < BN; r += NT) {
-          const int key = kt * BN + r;
-          bias[r] = key < s.nk && (!km || km[key]) ? 0.f : -INFINITY;
-        }
-      __syncthreads();
-      if (kt + 1 < nt) fetch(kt + 1);
-      if (!wave_live) continue;
-      auto p_dp = [&](int b, f32x16_t& sc, f32x16_t& dp) {       // p and dp of 32 keys
-        sc = mma_row<T, HDP>(Ks, LD, b * 32, qf, lane);
-        dp = mma_row<T, HDP>(Vs, LD, b * 32, df, lane);
-        if (masked) {
+      const T *Ks, *Vs;
+      const float* bias;
+      const bool masked = kt_.next(kt, nt, tid, Ks, Vs, bias);
+      if (wave_live) {
+        auto p_dp = [&](int b, f32x16_t& sc, f32x16_t& dp) {     // p and dp of 32 keys
+          sc = mma_row<T, HDP>(Ks, LD, b * 32, qf, lane);
+          dp = mma_row<T, HDP>(Vs, LD, b * 32, df, lane);
+          if (masked) mask_keys(sc, bias + b * 32, h);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float4 bi = *reinterpret_cast<const float4*>(bias + b * 32 + 8 * i + 4 * h);
-            sc[4 * i] = bi.x < 0.f ? -INFINITY : sc[4 * i]; sc[4 * i + 1] = bi.y < 0.f ? -INFINITY : sc[4 * i + 1];
-            sc[4 * i + 2] = bi.z < 0.f ? -INFINITY : sc[4 * i + 2]; sc[4 * i + 3] = bi.w < 0.f ? -INFINITY : sc[4 * i + 3];
+          for (int i = 0; i < 16; ++i) sc[i] = exp2_fast(fmaf(sc[i], c, -lse2));
+        };
+        if (sizeof(T) == 2 && nt == 1) {
+          // all keys are here: D = sum p dp, which is sum(do o) before o was rounded.  With a few keys dp - D cancels, and the rounding of o
+          // alone would double the error of dq and dk (two keys: 3.6e-3 instead of 2.4e-3 of their norm); over many keys |o| is small against |v|.
+          D = 0.f;
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            f32x16_t sc, dp;
+            p_dp(b, sc, dp);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) D = fmaf(sc[i], dp[i], D);
           }
+          D += other_half(D);
+          if (live && h == 0) p.delta[stat] = D;
         }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sc[i] = exp2_fast(fmaf(sc[i], c, -lse2));
-      };
-      if (sizeof(T) == 2 && nt == 1) {
-        // all keys are here: D = sum p dp, which is sum(do o) before o was rounded.  With a few keys dp - D cancels, and the rounding of o
-        // alone would double the error of dq and dk (two keys: 3.6e-3 instead of 2.4e-3 of their norm); over many keys |o| is small against |v|.
-        D = 0.f;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
           f32x16_t sc, dp;
           p_dp(b, sc, dp);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) D = fmaf(sc[i], dp[i], D);
+          for (int i = 0; i < 16; ++i) sc[i] *= dp[i] - D;
+          const typename Op<T>::PF pf = Op<T>::pack(sc);
+#pragma unroll
+          for (int d = 0; d < DB; ++d) Op<T>::mma_t(dq[d], Ks, LD, b * 32, d * 32, pf, lane);
         }
-        D += __shfl_xor(D, 32, 64);
-        if (live && h == 0) p.delta[stat] = D;
       }
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        f32x16_t sc, dp;
-        p_dp(b, sc, dp);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sc[i] *= dp[i] - D;
-        const typename Op<T>::PF pf = Op<T>::pack(sc);
-#pragma unroll
-        for (int d = 0; d < DB; ++d) Op<T>::mma_t(dq[d], Ks, LD, b * 32, d * 32, pf, lane);
-      }
+      __syncthreads();
     }
     if (live) {
       T* row = (T*)p.dq + m_offset(p, s, w.g, m, p.lddq);
@@ -531,13 +583,11 @@ __global__ __launch_bounds__(64 * NW) void xattn_dq_kernel(XP p) {
 
 // ------------------------------------------------------------------------------------------ backward: dk, dv
 template <typename T, int HDP, int NW, int BQ>
-__global__ __launch_bounds__(64 * NW) void xattn_dkv_kernel(XP p) {
+__global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(T) * HDP <= 128 ? 2 : 1) void xattn_dkv_kernel(XP p) {
   constexpr int EPC = Op<T>::EPC, LD = HDP + EPC, KS = HDP / (2 * EPC), DB = HDP / 32, NB = BQ / 32, BK = 32 * NW, NT = 64 * NW;
   DH_DYN_LDS_A16(unsigned char, smem);
-  T* Qs = reinterpret_cast<T*>(smem);
-  T* Ds = Qs + BQ * LD;
-  float* lse2s = reinterpret_cast<float*>(Ds + BQ * LD);
-  float* dels = lse2s + BQ;
+  T* buf = reinterpret_cast<T*>(smem);                 // two buffers of Q and dO rows, lse and D of the rows
+  float* stats = reinterpret_cast<float*>(buf + 4 * BQ * LD);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
   if ((int)blockIdx.x >= p.main_blocks) {
     int first, last;
@@ -565,50 +615,62 @@ __global__ __launch_bounds__(64 * NW) void xattn_dkv_kernel(XP p) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) dk[d][i] = dv[d][i] = 0.f;
     Pair2<T, HDP, BQ, NT> st;
+    float nlse = 0.f, ndel = 0.f;
     auto fetch = [&](int mt) {
-      st.fetch([&](int r) -> const T* { const int m = mt * BQ + r; return m < M ? (const T*)p.q + m_offset(p, s, w.g, m, p.ldq) : nullptr; },
-               [&](int r) -> const T* { return (const T*)p.dout + m_offset(p, s, w.g, mt * BQ + r, p.lddo); }, p.hd, tid);
+      st.fetch((const T*)p.q, (const T*)p.dout, [&](int m) { return m_offset(p, s, w.g, m, p.ldq); }, [&](int m) { return m_offset(p, s, w.g, m, p.lddo); },
+               mt * BQ, M - 1, nullptr, p.hd, tid);
+      if (tid < BQ) {
+        const long stat = m_stat(p, s, w.g, min(mt * BQ + tid, M - 1));
+        nlse = p.lse[stat];
+        ndel = p.delta[stat];
+      }
+    };
+    auto store = [&](int mt) {
+      T* b = buf + (mt & 1) * 2 * BQ * LD;
+      st.store(b, b + BQ * LD, (mt + 1) * BQ > M || p.hd < HDP, mt * BQ, M - 1, false, p.hd, tid);
+      if (tid < BQ) {
+        float* x = stats + (mt & 1) * 2 * BQ + tid;
+        x[0] = mt * BQ + tid < M && nlse != -INFINITY ? nlse * kLog2e : INFINITY;      // rows that are none, rows without a key: p = 0
+        x[BQ] = ndel;
+      }
     };
     const int n_mt = block_live ? nt : 0;
-    if (n_mt > 0) fetch(0);
+    if (n_mt > 0) {
+      fetch(0);
+      store(0);
+      if (n_mt > 1) fetch(1);
+      __syncthreads();
+    }
     for (int mt = 0; mt < n_mt; ++mt) {
-      __syncthreads();
-      st.store(Qs, Ds, [](int) { return false; }, tid);
-      for (int r = tid; r < BQ; r += NT) {
-        const int m = mt * BQ + r;
-        float a = INFINITY, d = 0.f;
-        if (m < M) {
-          const long stat = m_stat(p, s, w.g, m);
-          const float lse = p.lse[stat];
-          a = lse == -INFINITY ? INFINITY : lse * kLog2e;
-          d = p.delta[stat];
+      if (mt + 1 < n_mt) {
+        store(mt + 1);
+        if (mt + 2 < n_mt) fetch(mt + 2);
+      }
+      if (wave_live) {
+        const T *Qs = buf + (mt & 1) * 2 * BQ * LD, *Ds = Qs + BQ * LD;
+        const float *lse2s = stats + (mt & 1) * 2 * BQ, *dels = lse2s + BQ;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          f32x16_t sc = mma_row<T, HDP>(Qs, LD, b * 32, kf, lane);
+          f32x16_t dp = mma_row<T, HDP>(Ds, LD, b * 32, vf, lane);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float4 L = *reinterpret_cast<const float4*>(lse2s + b * 32 + 8 * i + 4 * h);
+            const float4 D = *reinterpret_cast<const float4*>(dels + b * 32 + 8 * i + 4 * h);
+            sc[4 * i] = exp2_fast(fmaf(sc[4 * i], c, -L.x)); dp[4 * i] = sc[4 * i] * (dp[4 * i] - D.x);
+            sc[4 * i + 1] = exp2_fast(fmaf(sc[4 * i + 1], c, -L.y)); dp[4 * i + 1] = sc[4 * i + 1] * (dp[4 * i + 1] - D.y);
+            sc[4 * i + 2] = exp2_fast(fmaf(sc[4 * i + 2], c, -L.z)); dp[4 * i + 2] = sc[4 * i + 2] * (dp[4 * i + 2] - D.z);
+            sc[4 * i + 3] = exp2_fast(fmaf(sc[4 * i + 3], c, -L.w)); dp[4 * i + 3] = sc[4 * i + 3] * (dp[4 * i + 3] - D.w);
+          }
+          const typename Op<T>::PF pf = Op<T>::pack(sc), sf = Op<T>::pack(dp);
+#pragma unroll
+          for (int d = 0; d < DB; ++d) {
+            Op<T>::mma_t(dv[d], Ds, LD, b * 32, d * 32, pf, lane);
+            Op<T>::mma_t(dk[d], Qs, LD, b * 32, d * 32, sf, lane);
+          }
         }
-        lse2s[r] = a;
-        dels[r] = d;
       }
       __syncthreads();
-      if (mt + 1 < n_mt) fetch(mt + 1);
-      if (!wave_live) continue;
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        f32x16_t sc = mma_row<T, HDP>(Qs, LD, b * 32, kf, lane);
-        f32x16_t dp = mma_row<T, HDP>(Ds, LD, b * 32, vf, lane);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float4 L = *reinterpret_cast<const float4*>(lse2s + b * 32 + 8 * i + 4 * h);
-          const float4 D = *reinterpret_cast<const float4*>(dels + b * 32 + 8 * i + 4 * h);
-          sc[4 * i] = exp2_fast(fmaf(sc[4 * i], c, -L.x)); dp[4 * i] = sc[4 * i] * (dp[4 * i] - D.x);
-          sc[4 * i + 1] = exp2_fast(fmaf(sc[4 * i + 1], c, -L.y)); dp[4 * i + 1] = sc[4 * i + 1] * (dp[4 * i + 1] - D.y);
-          sc[4 * i + 2] = exp2_fast(fmaf(sc[4 * i + 2], c, -L.z)); dp[4 * i + 2] = sc[4 * i + 2] * (dp[4 * i + 2] - D.z);
-          sc[4 * i + 3] = exp2_fast(fmaf(sc[4 * i + 3], c, -L.w)); dp[4 * i + 3] = sc[4 * i + 3] * (dp[4 * i + 3] - D.w);
-        }
-        const typename Op<T>::PF pf = Op<T>::pack(sc), sf = Op<T>::pack(dp);
-#pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          Op<T>::mma_t(dv[d], Ds, LD, b * 32, d * 32, pf, lane);
-          Op<T>::mma_t(dk[d], Qs, LD, b * 32, d * 32, sf, lane);
-        }
-      }
     }
     if (in) {
       T* krow = (T*)p.dk + (long)(s.k0 + key) * p.lddk + (long)w.g * p.hd;
@@ -650,16 +712,18 @@ int length_hint(int given, const int* cu, int rows, int batch) {
   return (int)(n > rows ? rows : n);
 }
 
+// heads of more than 64 columns, bf16, many rows: 8 waves share a tile (half the staging registers each, so two waves fit a SIMD)
+bool wide_block(const dh_xattn_args* a, int64_t mq) { return a->dtype == DH_BF16 && a->hd > 64 && mq > 128; }
 struct Plan { int nw, bn, tiles, nsplit; };
 Plan plan_fwd(const dh_xattn_args* a) {
   const int rep = a->heads / a->kv_heads;
   const int64_t mq = (int64_t)length_hint(a->max_q, a->cu_q, a->rows_q, a->batch) * rep;
   const int mk = length_hint(a->max_kv, a->cu_kv, a->rows_kv, a->batch);
   Plan r;
-  r.nw = mq <= 32 ? 1 : 4;
+  r.nw = mq <= 32 ? 1 : wide_block(a, mq) ? 8 : 4;
   r.bn = (r.nw == 1 || a->dtype == DH_F32) ? 32 : 64;
   r.tiles = (int)cdiv64(mq < 1 ? 1 : mq, 32 * r.nw);
-  const int64_t blocks = (int64_t)r.tiles * a->batch * a->kv_heads, want = (int64_t)x_cus() * (r.nw == 1 ? 8 : 2);
+  const int64_t blocks = (int64_t)r.tiles * a->batch * a->kv_heads, want = (int64_t)x_cus() * (8 / r.nw);
   int64_t ns = blocks >= want ? 1 : want / blocks;
   const int64_t most = cdiv64(mk, 4 * r.bn);          // a range is at least four tiles long
   if (ns > most) ns = most;
@@ -702,6 +766,7 @@ XP params(const dh_xattn_args* a) {
   p.ldq = a->ldq; p.ldk = a->ldk; p.ldv = a->ldv; p.ldo = a->ldo; p.lddo = a->lddo; p.lddq = a->lddq; p.lddk = a->lddk; p.lddv = a->lddv;
   p.rows_q = a->rows_q; p.rows_kv = a->rows_kv; p.batch = a->batch; p.heads = a->heads; p.kv_heads = a->kv_heads; p.rep = a->heads / a->kv_heads; p.hd = a->hd;
   p.scale = a->scale;
+  p.magic = p.rep > 1 ? (unsigned)(((1ull << 32) + p.rep - 1) / p.rep) : 0u;
   p.nsplit = 1;
   return p;
 }
@@ -727,13 +792,17 @@ int launch(K kernel, const XP& p, int64_t grid, int threads, size_t lds, hipStre
   return DH_OK;
 }
 
-template <typename T, int HDP> constexpr size_t tile_bytes(int rows) { return (size_t)2 * rows * (HDP + Op<T>::EPC) * sizeof(T); }
+// two buffers of two tiles, `per_row` floats beside each tile row
+template <typename T, int HDP> constexpr size_t tile_bytes(int rows, int per_row) { return 2 * ((size_t)2 * rows * (HDP + Op<T>::EPC) * sizeof(T) + (size_t)rows * per_row * 4); }
 
 template <typename T, int HDP>
 int fwd_hd(XP& p, const Plan& pl, int64_t grid, hipStream_t st) {
   constexpr int BN = sizeof(T) == 2 ? 64 : 32;
-  const size_t lds1 = tile_bytes<T, HDP>(32) + 32 * 4, lds4 = tile_bytes<T, HDP>(BN) + BN * 4;
+  const size_t lds1 = tile_bytes<T, HDP>(32, 1), lds4 = tile_bytes<T, HDP>(BN, 1);
   if (pl.nw == 1) return pl.nsplit > 1 ? launch(xattn_fwd_kernel<T, HDP, 1, 32, true>, p, grid, 64, lds1, st) : launch(xattn_fwd_kernel<T, HDP, 1, 32, false>, p, grid, 64, lds1, st);
+  if constexpr (sizeof(T) == 2 && HDP > 64) {
+    if (pl.nw == 8) return pl.nsplit > 1 ? launch(xattn_fwd_kernel<T, HDP, 8, BN, true>, p, grid, 512, lds4, st) : launch(xattn_fwd_kernel<T, HDP, 8, BN, false>, p, grid, 512, lds4, st);
+  }
   return pl.nsplit > 1 ? launch(xattn_fwd_kernel<T, HDP, 4, BN, true>, p, grid, 256, lds4, st) : launch(xattn_fwd_kernel<T, HDP, 4, BN, false>, p, grid, 256, lds4, st);
 }
 template <typename T, int HDP>
@@ -742,12 +811,23 @@ int bwd_hd(XP& p, const dh_xattn_args* a, hipStream_t st) {
   int64_t grid;
   const int64_t mq = (int64_t)length_hint(a->max_q, a->cu_q, a->rows_q, a->batch) * p.rep;
   if (a->rows_q > 0) {
-    if (int e = lay_out(p, (int)cdiv64(mq, 128), 1, a->cu_q != nullptr, grid)) return e;
-    if (int e = launch(xattn_dq_kernel<T, HDP, 4, BN>, p, grid, 256, tile_bytes<T, HDP>(BN) + BN * 4, st)) return e;
+    const bool wide = wide_block(a, mq);
+    if (int e = lay_out(p, (int)cdiv64(mq, wide ? 256 : 128), 1, a->cu_q != nullptr, grid)) return e;
+    if constexpr (sizeof(T) == 2 && HDP > 64) {
+      if (wide)
+        if (int e = launch(xattn_dq_kernel<T, HDP, 8, BN>, p, grid, 512, tile_bytes<T, HDP>(BN, 1), st)) return e;
+    }
+    if (!wide)
+      if (int e = launch(xattn_dq_kernel<T, HDP, 4, BN>, p, grid, 256, tile_bytes<T, HDP>(BN, 1), st)) return e;
   }
   if (a->rows_kv > 0) {
-    if (int e = lay_out(p, (int)cdiv64(length_hint(a->max_kv, a->cu_kv, a->rows_kv, a->batch), 128), 1, a->cu_kv != nullptr, grid)) return e;
-    if (int e = launch(xattn_dkv_kernel<T, HDP, 4, 32>, p, grid, 256, tile_bytes<T, HDP>(32) + 32 * 8, st)) return e;
+    const int mk = length_hint(a->max_kv, a->cu_kv, a->rows_kv, a->batch);
+    const bool wide = a->dtype == DH_BF16 && a->hd > 64 && mk > 128;
+    if (int e = lay_out(p, (int)cdiv64(mk, wide ? 256 : 128), 1, a->cu_kv != nullptr, grid)) return e;
+    if constexpr (sizeof(T) == 2 && HDP > 64) {
+      if (wide) return launch(xattn_dkv_kernel<T, HDP, 8, 32>, p, grid, 512, tile_bytes<T, HDP>(32, 2), st);
+    }
+    return launch(xattn_dkv_kernel<T, HDP, 4, 32>, p, grid, 256, tile_bytes<T, HDP>(32, 2), st);
   }
   return DH_OK;
 }

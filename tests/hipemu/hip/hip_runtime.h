@@ -51,6 +51,7 @@ static inline int __float_as_int(float f) { int u; memcpy(&u, &f, 4); return u; 
 #define __builtin_amdgcn_exp2f(x) exp2f(x)
 static inline float cospif(float x) { return (float)cos(M_PI * (double)x); }
 static inline float sinpif(float x) { return (float)sin(M_PI * (double)x); }
+static inline unsigned __umulhi(unsigned a, unsigned b) { return (unsigned)(((uint64_t)a * b) >> 32); }
 static inline float rsqrtf(float x) { return 1.f / sqrtf(x); }
 static inline float __frcp_rn(float x) { return 1.f / x; }
 static inline float __fdividef(float a, float b) { return a / b; }
@@ -80,6 +81,12 @@ static inline T __shfl(T v, int src, int width = 64) {
   T r;
   memcpy(&r, all + (size_t)(src & 63) * sizeof(T), sizeof(T));
   return r;
+}
+static inline int __any(int pred) {                     // (every lane of the wave has to call it; lanes that have left deposit nothing)
+  int any = 0;
+  for (int m = 32; m; m >>= 1) pred |= __shfl_xor(pred, m);
+  any = pred;
+  return any;
 }
 // lanes of a wave run in lockstep on the hardware; here they are independent fibers, so a wave barrier must really wait
 static inline void emu_wave_barrier() { const char c = 0; (void)emu_wave_gather(&c, 1); }
