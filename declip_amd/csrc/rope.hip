@@ -11,7 +11,7 @@
 
 namespace {
 
-constexpr int MAX_PAIRS = 128;
+constexpr int MAX_PAIRS = DH_ROPE_MAX_PAIRS;
 struct RopeP {
   const void* x;
   void* y;
@@ -124,32 +124,45 @@ int rope_launch(const RopeP& p, hipStream_t st) {
 
 }  // namespace
 
-extern "C" int dh_rope_axes(int dtype, const void* x, int64_t ldx, void* y, int64_t ldy, int rows, int heads, int hd, const void* pos,
-                            int pos_float, int pos_rows, const int* sections, const double* theta, int axes, int joint, int interleaved, int inverse,
-                            dh_stream_t stream) {
-  DH_REQUIRE(dtype == DH_F32 || dtype == DH_BF16, "dh_rope_axes: dtype %d", dtype);
-  DH_REQUIRE(rows >= 0 && heads > 0 && hd > 0 && axes > 0 && axes <= 8 && sections && theta, "dh_rope_axes: rows %d, heads %d, head size %d, axes %d", rows, heads, hd, axes);
+extern "C" int dh_rope_plan_init(dh_rope_plan* plan, int hd, const int* sections, const double* theta, int axes, int joint, int interleaved) {
+  DH_REQUIRE(plan && sections && theta, "dh_rope_plan_init: null pointer");
+  DH_REQUIRE(hd > 0 && axes > 0 && axes <= 8, "dh_rope_plan_init: head size %d, %d axes (up to 8)", hd, axes);
   int64_t pairs = 0;
   for (int a = 0; a < axes; ++a) {
-    DH_REQUIRE(sections[a] > 0 && sections[a] <= MAX_PAIRS, "dh_rope_axes: section %d of axis %d", sections[a], a);
-    DH_REQUIRE(theta[a] > 0. && theta[a] < INFINITY, "dh_rope_axes: theta of axis %d must be positive and finite", a);
-    DH_REQUIRE(!joint || theta[a] == theta[0], "dh_rope_axes: a joint ladder has one theta");
+    DH_REQUIRE(sections[a] > 0 && sections[a] <= MAX_PAIRS, "dh_rope_plan_init: section %d of axis %d", sections[a], a);
+    DH_REQUIRE(theta[a] > 0. && theta[a] < INFINITY, "dh_rope_plan_init: theta of axis %d must be positive and finite", a);
+    DH_REQUIRE(!joint || theta[a] == theta[0], "dh_rope_plan_init: a joint ladder has one theta");
     pairs += sections[a];
   }
-  DH_REQUIRE(pairs <= MAX_PAIRS && 2 * pairs <= hd, "dh_rope_axes: %lld pairs in a head of %d", (long long)pairs, hd);
-  DH_REQUIRE(ldx >= (int64_t)heads * hd && ldy >= (int64_t)heads * hd, "dh_rope_axes: row strides %lld, %lld for %d heads of %d", (long long)ldx, (long long)ldy, heads, hd);
-  if (rows == 0) return DH_OK;
-  DH_REQUIRE(x && y && pos && pos_rows > 0 && rows % pos_rows == 0, "dh_rope_axes: %d rows, %d positions", rows, pos_rows);
-  RopeP p;
-  p.x = x; p.y = y; p.pos = pos; p.ldx = ldx; p.ldy = ldy;
-  p.rows = rows; p.pos_rows = pos_rows; p.axes = axes; p.heads = heads; p.hd = hd; p.pairs = (int)pairs; p.interleaved = interleaved; p.frac = pos_float;
-  p.sign = inverse ? -1.f : 1.f;
+  DH_REQUIRE(pairs <= MAX_PAIRS && 2 * pairs <= hd, "dh_rope_plan_init: %lld pairs in a head of %d", (long long)pairs, hd);
+  plan->axes = axes; plan->pairs = (int)pairs; plan->hd = hd; plan->interleaved = interleaved != 0;
   int k = 0;
   for (int a = 0; a < axes; ++a)
     for (int j = 0; j < sections[a]; ++j, ++k) {
       const double e = joint ? (double)k / (double)pairs : (double)j / (double)sections[a];
-      p.f[k] = pow(theta[a], -e) / 6.283185307179586476925286766559;
-      p.axis[k] = (unsigned char)a;
+      plan->turns[k] = pow(theta[a], -e) / 6.283185307179586476925286766559;
+      plan->axis[k] = (unsigned char)a;
     }
+  return DH_OK;
+}
+
+extern "C" int dh_rope_axes(const dh_rope_plan* plan, int dtype, const void* x, int64_t ldx, void* y, int64_t ldy, int rows, int heads, const void* pos,
+                            int pos_float, int pos_rows, int inverse, dh_stream_t stream) {
+  DH_REQUIRE(plan && plan->axes > 0 && plan->axes <= 8 && plan->pairs > 0 && plan->pairs <= MAX_PAIRS && plan->hd >= 2 * plan->pairs, "dh_rope_axes: plan not initialised");
+  DH_REQUIRE(dtype == DH_F32 || dtype == DH_BF16, "dh_rope_axes: dtype %d", dtype);
+  DH_REQUIRE(rows >= 0 && heads > 0, "dh_rope_axes: rows %d, heads %d", rows, heads);
+  const int64_t width = (int64_t)heads * plan->hd;
+  DH_REQUIRE(width < (1 << 30) && (rows <= 1 || (ldx >= width && ldy >= width)), "dh_rope_axes: row strides %lld, %lld for %d heads of %d", (long long)ldx, (long long)ldy, heads, plan->hd);
+  if (rows == 0) return DH_OK;
+  DH_REQUIRE(x && y && pos && pos_rows > 0 && rows % pos_rows == 0, "dh_rope_axes: %d rows, %d positions", rows, pos_rows);
+  RopeP p;
+  p.x = x; p.y = y; p.pos = pos; p.ldx = ldx; p.ldy = ldy;
+  p.rows = rows; p.pos_rows = pos_rows; p.axes = plan->axes; p.heads = heads; p.hd = plan->hd; p.pairs = plan->pairs; p.interleaved = plan->interleaved; p.frac = pos_float;
+  p.sign = inverse ? -1.f : 1.f;
+  for (int k = 0; k < p.pairs; ++k) {
+    DH_REQUIRE(plan->axis[k] < plan->axes, "dh_rope_axes: plan not initialised");
+    p.f[k] = plan->turns[k];
+    p.axis[k] = plan->axis[k];
+  }
   return dtype == DH_BF16 ? rope_launch<bf16_t>(p, (hipStream_t)stream) : rope_launch<float>(p, (hipStream_t)stream);
 }

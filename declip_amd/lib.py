@@ -67,6 +67,11 @@ class XattnArgs(Structure):
                 + [(n, c_void_p) for n in ("cu_q", "cu_kv", "kv_len", "key_mask", "ws")] + [("ws_bytes", c_int64)])
 
 
+class RopePlan(Structure):
+    """dh_rope_plan (include/declip_hip.h)"""
+    _fields_ = [(n, c_int) for n in ("axes", "pairs", "hd", "interleaved")] + [("turns", c_double * 128), ("axis", ctypes.c_ubyte * 128)]
+
+
 class JoinNormArgs(Structure):
     """dh_join_norm_args (include/declip_hip.h)"""
     _fields_ = ([(n, c_int) for n in ("dtype", "rows", "d", "rms", "gate_rows", "gate_channel", "gate_tanh")] + [("alpha", c_float), ("eps", c_float)]
@@ -112,7 +117,8 @@ _PROTOS = {
     "dh_xattn_ws_bytes": (c_int64, [POINTER(XattnArgs), c_int]),
     "dh_xattn_fwd": (c_int, [POINTER(XattnArgs), _P]),
     "dh_xattn_bwd": (c_int, [POINTER(XattnArgs), _P]),
-    "dh_rope_axes": (c_int, [c_int, _P, c_int64, _P, c_int64, c_int, c_int, c_int, _P, c_int, c_int, POINTER(c_int), POINTER(c_double), c_int, c_int, c_int, c_int, _P]),
+    "dh_rope_plan_init": (c_int, [POINTER(RopePlan), c_int, POINTER(c_int), POINTER(c_double), c_int, c_int, c_int]),
+    "dh_rope_axes": (c_int, [POINTER(RopePlan), c_int, _P, c_int64, _P, c_int64, c_int, c_int, _P, c_int, c_int, c_int, _P]),
     "dh_join_norm_fwd": (c_int, [POINTER(JoinNormArgs), _P]),
     "dh_join_norm_bwd_ws_bytes": (c_int64, [POINTER(JoinNormArgs)]),
     "dh_join_norm_bwd": (c_int, [POINTER(JoinNormArgs), _P]),

@@ -4,7 +4,6 @@ These only validate shapes, allocate outputs with torch (memory plumbing) and en
 HIP kernel on torch's current stream.  No arithmetic happens in Python/PyTorch here.
 """
 import collections
-import contextlib
 import ctypes
 
 import torch
@@ -872,36 +871,65 @@ def attnpool_tokens_bwd(dtok, dpos, b, HW):
 # ---------------------------------------------------------------------------------------------
 # operators between the towers (csrc/xattn.hip, rope.hip, join_norm.hip); their autograd functions: declip_amd/fusion.py
 # ---------------------------------------------------------------------------------------------
-def _on_device_of(t, *others):
-    """All tensors of a call lie on one device; the launch goes to that device and its current stream, whatever the current device is."""
+# A call's shapes, strides and options are checked once and kept as a filled argument struct ("plan"), found again by those values; what is left of a call is the
+# devices, the tables and the pointers.  Serving calls take a few microseconds on the device: 25 us of checks in front of each were most of their time.
+_PLANS = {}
+
+
+def _plan(key, make):
+    plan = _PLANS.get(key)
+    if plan is None:
+        plan = make()
+        if len(_PLANS) > 1024:
+            _PLANS.clear()
+        _PLANS[key] = plan
+    return plan
+
+
+def _device_of(t, *others):
+    """the device index of a call's tensors (-1: not on a HIP device, which ptr() refuses); all of them lie on one device"""
+    dev = t.get_device()
     for o in others:
-        _req(o is None or o.device == t.device, "tensors on different devices (%s, %s)" % (t.device, None if o is None else o.device))
-    if t.is_cuda and t.device.index != torch.cuda.current_device():
-        return torch.cuda.device(t.device)
-    return contextlib.nullcontext()
+        if o is not None and (o.get_device() != dev or o.is_meta):
+            raise L.DeclipHipError("bad argument: tensors on different devices (%s, %s)" % (t.device, o.device))
+    if dev < 0:
+        ptr(t)
+    return dev
 
 
-def _rows2d(t, name, width=None):
+def _elsewhere(dev):
+    """the launch goes to the tensors' device and its current stream: True if that is not the current device"""
+    return dev >= 0 and dev != torch.cuda.current_device()
+
+
+def _stream_on(dev):
+    return torch._C._cuda_getCurrentRawStream(dev) if dev >= 0 else stream()
+
+
+def _row_stride(t, name, width=None):
     """a [rows, width] tensor with contiguous columns -> its row stride in elements"""
     _req(t.dim() == 2 and (width is None or t.shape[1] == width) and (t.shape[1] == 1 or t.stride(1) == 1),
          "%s: [rows, %s] with contiguous columns" % (name, "width" if width is None else width))
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _table(t, name, n):
-    _req(t is None or (t.dtype == torch.int32 and t.numel() == n and t.is_contiguous()), "%s: contiguous int32 [%d]" % (name, n))
-    return t
+def _i32_table(t, name, n):
+    if t is None:
+        return None
+    if t.dtype is not torch.int32 or t.numel() != n or not t.is_contiguous():
+        raise L.DeclipHipError("bad argument: %s: contiguous int32 [%d]" % (name, n))
+    return t.data_ptr()
 
 
-def _xattn_args(q, k, v, heads, kv_heads, batch, cu_q, cu_kv, kv_len, key_mask, scale, max_q, max_kv):
+def _xattn_plan(q, k, v, heads, kv_heads, batch, n_q, n_kv, scale, max_q, max_kv):
     heads = int(heads)
     kv_heads = heads if kv_heads is None else int(kv_heads)
     _req(q.dim() == 2 and heads > 0 and kv_heads > 0 and heads % kv_heads == 0 and q.shape[1] % heads == 0, "q [rows, heads * hd], heads a multiple of kv_heads")
     hd = q.shape[1] // heads
-    for n in (cu_q, cu_kv):
+    for n in (n_q, n_kv):
         if n is not None:
-            _req(n.numel() >= 2 and (batch is None or batch == n.numel() - 1), "cu_q / cu_kv [batch + 1]")
-            batch = n.numel() - 1
+            _req(n >= 2 and (batch is None or batch == n - 1), "cu_q / cu_kv [batch + 1]")
+            batch = n - 1
     _req(batch is not None and batch > 0, "batch: the number of sequences (or a cu_q / cu_kv table)")
     _req(q.dtype == k.dtype == v.dtype, "q, k, v of one dtype")
     _req(k.shape == v.shape, "k and v of one shape")
@@ -909,14 +937,33 @@ def _xattn_args(q, k, v, heads, kv_heads, batch, cu_q, cu_kv, kv_len, key_mask, 
     a.dtype, a.batch, a.heads, a.kv_heads, a.hd = dt(q), int(batch), heads, kv_heads, hd
     a.rows_q, a.rows_kv, a.max_q, a.max_kv = q.shape[0], k.shape[0], int(max_q or 0), int(max_kv or 0)
     a.scale = float(scale) if scale is not None else hd ** -0.5
-    a.ldq, a.ldk, a.ldv = _rows2d(q, "q"), _rows2d(k, "k", kv_heads * hd), _rows2d(v, "v", kv_heads * hd)
-    a.q, a.k, a.v = ptr(q), ptr(k), ptr(v)
-    a.cu_q, a.cu_kv = ptr(_table(cu_q, "cu_q", a.batch + 1)), ptr(_table(cu_kv, "cu_kv", a.batch + 1))
-    a.kv_len = ptr(_table(kv_len, "kv_len", a.batch))
+    a.ldq, a.ldk, a.ldv = _row_stride(q, "q"), _row_stride(k, "k", kv_heads * hd), _row_stride(v, "v", kv_heads * hd)
+    a.ldo = a.lddo = a.lddq = q.shape[1]
+    a.lddk = a.lddv = k.shape[1]
+    # the tables' presence decides the workspace, their place does not
+    probe = L.XattnArgs.from_buffer_copy(a)
+    probe.cu_q, probe.cu_kv = (None if n is None else 16 for n in (n_q, n_kv))
+    need = L.load().dh_xattn_ws_bytes(ctypes.byref(probe), 0)
+    return a, max(int(need), 0)
+
+
+def _xattn_call(q, k, v, heads, kv_heads, batch, cu_q, cu_kv, kv_len, key_mask, scale, max_q, max_kv):
+    n_q, n_kv = None if cu_q is None else cu_q.numel(), None if cu_kv is None else cu_kv.numel()
+    key = ("xattn", q.dtype, k.dtype, v.dtype, q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), heads, kv_heads, batch, n_q, n_kv, scale, max_q, max_kv)
+    plan, need = _plan(key, lambda: _xattn_plan(q, k, v, heads, kv_heads, batch, n_q, n_kv, scale, max_q, max_kv))
+    a = L.XattnArgs.from_buffer_copy(plan)
+    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if cu_q is not None:
+        a.cu_q = _i32_table(cu_q, "cu_q", a.batch + 1)
+    if cu_kv is not None:
+        a.cu_kv = _i32_table(cu_kv, "cu_kv", a.batch + 1)
+    if kv_len is not None:
+        a.kv_len = _i32_table(kv_len, "kv_len", a.batch)
     if key_mask is not None:
-        _req(key_mask.dtype in (torch.bool, torch.uint8) and key_mask.numel() == a.rows_kv and key_mask.is_contiguous(), "key_mask: contiguous bool / uint8, one per key row")
-        a.key_mask = ptr(key_mask)
-    return a
+        if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.numel() != a.rows_kv or not key_mask.is_contiguous():
+            raise L.DeclipHipError("bad argument: key_mask: contiguous bool / uint8, one per key row")
+        a.key_mask = key_mask.data_ptr()
+    return a, need
 
 
 def xattn_fwd(q, k, v, heads, *, kv_heads=None, batch=None, cu_q=None, cu_kv=None, kv_len=None, key_mask=None, scale=None, max_q=None, max_kv=None):
@@ -925,36 +972,57 @@ def xattn_fwd(q, k, v, heads, *, kv_heads=None, batch=None, cu_q=None, cu_kv=Non
     Sequence i: query rows cu_q[i] .. cu_q[i+1], key rows cu_kv[i] .. cu_kv[i+1] (int32, on the device; None: `batch` equal parts), of which the first
     kv_len[i] (None: all) with key_mask != 0 (None: all) are keys.  No key: out = 0, lse = -inf.  hd: a multiple of 8 up to 128; max_q / max_kv: the
     longest sequence if the caller knows it (grid layout only).  scale: hd ** -0.5."""
-    with _on_device_of(q, k, v, cu_q, cu_kv, kv_len, key_mask):
-        a = _xattn_args(q, k, v, heads, kv_heads, batch, cu_q, cu_kv, kv_len, key_mask, scale, max_q, max_kv)
-        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        lse = torch.empty(a.heads, a.rows_q, device=q.device, dtype=torch.float32)
-        a.out, a.ldo, a.lse = ptr(out), out.shape[1], ptr(lse)
-        lib = L.load()
-        need = lib.dh_xattn_ws_bytes(ctypes.byref(a), 0)
-        if need > 0:
-            ws = torch.empty(need // 4, device=q.device, dtype=torch.float32)
-            a.ws, a.ws_bytes = ptr(ws), need
-        check(lib.dh_xattn_fwd(ctypes.byref(a), stream()), "dh_xattn_fwd")
+    dev = _device_of(q, k, v, cu_q, cu_kv, kv_len, key_mask)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return xattn_fwd(q, k, v, heads, kv_heads=kv_heads, batch=batch, cu_q=cu_q, cu_kv=cu_kv, kv_len=kv_len, key_mask=key_mask, scale=scale, max_q=max_q, max_kv=max_kv)
+    a, need = _xattn_call(q, k, v, heads, kv_heads, batch, cu_q, cu_kv, kv_len, key_mask, scale, max_q, max_kv)
+    on = q.device
+    out = torch.empty(a.rows_q, a.ldo, device=on, dtype=q.dtype)
+    lse = torch.empty(a.heads, a.rows_q, device=on, dtype=torch.float32)
+    a.out, a.lse = out.data_ptr(), lse.data_ptr()
+    if need:
+        ws = torch.empty(need // 4, device=on, dtype=torch.float32)
+        a.ws, a.ws_bytes = ws.data_ptr(), need
+    check(L.load().dh_xattn_fwd(ctypes.byref(a), _stream_on(dev)), "dh_xattn_fwd")
     return out, lse
 
 
 def xattn_bwd(q, k, v, out, dout, lse, heads, *, kv_heads=None, batch=None, cu_q=None, cu_kv=None, kv_len=None, key_mask=None, scale=None, max_q=None, max_kv=None):
     """Gradients of xattn_fwd (same geometry arguments; out, lse: its results) -> (dq, dk, dv), contiguous."""
-    with _on_device_of(q, k, v, out, dout, lse, cu_q, cu_kv, kv_len, key_mask):
-        a = _xattn_args(q, k, v, heads, kv_heads, batch, cu_q, cu_kv, kv_len, key_mask, scale, max_q, max_kv)
-        _req(out.shape == q.shape == dout.shape and out.dtype == q.dtype == dout.dtype, "out and dout like q")
-        _req(lse.shape == (a.heads, a.rows_q) and lse.dtype == torch.float32 and lse.is_contiguous(), "lse: contiguous fp32 [heads, rows_q]")
-        dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
-        a.out, a.ldo, a.lse = ptr(out), _rows2d(out, "out"), ptr(lse)
-        a.dout, a.lddo = ptr(dout), _rows2d(dout, "dout")
-        a.dq, a.lddq, a.dk, a.lddk, a.dv, a.lddv = ptr(dq), q.shape[1], ptr(dk), k.shape[1], ptr(dv), v.shape[1]
-        lib = L.load()
-        need = lib.dh_xattn_ws_bytes(ctypes.byref(a), 1)
-        ws = torch.empty(max(need, 16) // 4, device=q.device, dtype=torch.float32)
-        a.ws, a.ws_bytes = ptr(ws), need
-        check(lib.dh_xattn_bwd(ctypes.byref(a), stream()), "dh_xattn_bwd")
+    dev = _device_of(q, k, v, out, dout, lse, cu_q, cu_kv, kv_len, key_mask)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return xattn_bwd(q, k, v, out, dout, lse, heads, kv_heads=kv_heads, batch=batch, cu_q=cu_q, cu_kv=cu_kv, kv_len=kv_len, key_mask=key_mask, scale=scale,
+                             max_q=max_q, max_kv=max_kv)
+    a, _ = _xattn_call(q, k, v, heads, kv_heads, batch, cu_q, cu_kv, kv_len, key_mask, scale, max_q, max_kv)
+    if not (out.shape == q.shape == dout.shape and out.dtype == q.dtype == dout.dtype):
+        raise L.DeclipHipError("bad argument: out and dout like q")
+    if lse.shape != (a.heads, a.rows_q) or lse.dtype is not torch.float32 or not lse.is_contiguous():
+        raise L.DeclipHipError("bad argument: lse: contiguous fp32 [heads, rows_q]")
+    on = q.device
+    dq = torch.empty(a.rows_q, a.lddq, device=on, dtype=q.dtype)
+    dk, dv = (torch.empty(a.rows_kv, a.lddk, device=on, dtype=q.dtype) for _ in range(2))
+    ws = torch.empty(max(a.heads * a.rows_q, 4), device=on, dtype=torch.float32)      # = dh_xattn_ws_bytes(args, 1)
+    a.out, a.ldo, a.lse = out.data_ptr(), _row_stride(out, "out"), lse.data_ptr()
+    a.dout, a.lddo = dout.data_ptr(), _row_stride(dout, "dout")
+    a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    a.ws, a.ws_bytes = ws.data_ptr(), ws.numel() * 4
+    check(L.load().dh_xattn_bwd(ctypes.byref(a), _stream_on(dev)), "dh_xattn_bwd")
     return dq, dk, dv
+
+
+def _rope_plan(x, pos, heads, sections, theta, joint, interleaved):
+    _req(x.dim() == 2 and heads > 0 and x.shape[1] % heads == 0 and x.shape[1] > 0, "x [rows, heads * hd]")
+    _row_stride(x, "x")
+    dt(x)
+    _req(pos.dim() == 2 and pos.shape[1] == len(sections) and pos.dtype in (torch.int32, torch.float32), "pos: contiguous int32 / fp32 [rows, axes]")
+    ths = list(theta) if isinstance(theta, tuple) else [theta] * len(sections)
+    _req(len(ths) == len(sections), "theta: one, or one per axis")
+    n, plan = len(sections), L.RopePlan()
+    check(L.load().dh_rope_plan_init(ctypes.byref(plan), x.shape[1] // heads, (ctypes.c_int * n)(*sections), (ctypes.c_double * n)(*ths), n, int(joint), int(interleaved)),
+          "dh_rope_plan_init")
+    return ctypes.byref(plan), dt(x), x.shape[0], x.shape[1], pos.shape[0], int(pos.dtype == torch.float32)
 
 
 def rope_axes(x, pos, heads, sections, theta=10000.0, *, joint=False, interleaved=False, inverse=False, out=None):
@@ -962,89 +1030,114 @@ def rope_axes(x, pos, heads, sections, theta=10000.0, *, joint=False, interleave
     fp32; sections: pairs per axis (2 * sum <= hd, the rest of a head is copied); theta: one base, or one per axis; joint: one frequency ladder shared by
     the axes; interleaved: pairs of neighbouring columns instead of the two halves; inverse: rotate back (the gradient).  out: x itself (in
     place) or memory of its own."""
-    heads, sections = int(heads), [int(s) for s in sections]
-    with _on_device_of(x, pos, out):
-        ldx = _rows2d(x, "x")
-        _req(heads > 0 and x.shape[1] % heads == 0 and x.shape[1] > 0, "x [rows, heads * hd]")
-        _req(pos.dim() == 2 and pos.shape[1] == len(sections) and pos.is_contiguous() and pos.dtype in (torch.int32, torch.float32), "pos: contiguous int32 / fp32 [rows, axes]")
-        if out is None:
-            out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        else:
-            same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
-            _req(out.shape == x.shape and out.dtype == x.dtype and (same or out.untyped_storage().data_ptr() != x.untyped_storage().data_ptr()),
-                 "out: like x, x itself or memory of its own")
-        ths = [float(t) for t in theta] if isinstance(theta, (tuple, list)) else [float(theta)] * len(sections)
-        _req(len(ths) == len(sections), "theta: one, or one per axis")
-        n = len(sections)
-        check(L.load().dh_rope_axes(dt(x), ptr(x), ldx, ptr(out), _rows2d(out, "out"), x.shape[0], heads, x.shape[1] // heads, ptr(pos), int(pos.dtype == torch.float32),
-                                    pos.shape[0], (ctypes.c_int * n)(*sections), (ctypes.c_double * n)(*ths), n, int(joint), int(interleaved), int(inverse),
-                                    stream()), "dh_rope_axes")
+    dev = _device_of(x, pos, out)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return rope_axes(x, pos, heads, sections, theta, joint=joint, interleaved=interleaved, inverse=inverse, out=out)
+    sections = tuple(sections)
+    theta = tuple(theta) if isinstance(theta, (tuple, list)) else theta
+    key = ("rope", x.dtype, x.shape, x.stride(), pos.dtype, pos.shape, heads, sections, theta, joint, interleaved)
+    plan, d, rows, width, pos_rows, frac = _plan(key, lambda: _rope_plan(x, pos, heads, sections, theta, joint, interleaved))
+    if not pos.is_contiguous():
+        raise L.DeclipHipError("bad argument: pos: contiguous int32 / fp32 [rows, axes]")
+    ldx = x.stride(0) if rows > 1 else width
+    if out is None:
+        out, ldy = torch.empty(rows, width, device=x.device, dtype=x.dtype), width
+    else:
+        ldy = _row_stride(out, "out", width)
+        same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
+        _req(out.shape == x.shape and out.dtype == x.dtype and (same or out.untyped_storage().data_ptr() != x.untyped_storage().data_ptr()),
+             "out: like x, x itself or memory of its own")
+    check(L.load().dh_rope_axes(plan, d, x.data_ptr(), ldx, out.data_ptr(), ldy, rows, heads, pos.data_ptr(), frac, pos_rows, inverse, _stream_on(dev)), "dh_rope_axes")
     return out
 
 
 JoinNormGrads = collections.namedtuple("JoinNormGrads", "post_w post_b gate scale pre_w pre_b")
 
 
-def _join_args(x, y, post, gate, scale, pre, alpha, eps, rms, gate_tanh):
+def _join_plan(x, y, gate, rms, gate_tanh, alpha, eps):
     _req(x.dim() == 2 and x.shape == y.shape and x.dtype == y.dtype, "x and y [rows, d] of one dtype")
-    rows, d = x.shape
     a = L.JoinNormArgs()
-    a.dtype, a.rows, a.d, a.rms, a.gate_tanh, a.alpha, a.eps = dt(x), rows, d, int(rms), int(gate_tanh), float(alpha), float(eps)
-    a.x, a.y = ptr(_contig(x, "x")), ptr(_contig(y, "y"))
-
-    def vec(t, name):
-        _req(t is None or (t.dtype == torch.float32 and t.numel() == d and t.is_contiguous()), "%s: contiguous fp32 [d]" % name)
-        return ptr(t)
-
-    if post is not None:
-        a.post_w, a.post_b = vec(post[0], "post weight"), vec(post[1], "post bias")
-    if pre is not None:
-        a.pre_w, a.pre_b = vec(pre[0], "pre weight"), vec(pre[1], "pre bias")
-    a.scale = vec(scale, "scale")
+    a.dtype, a.rms, a.gate_tanh, a.alpha, a.eps = dt(x), int(rms), int(gate_tanh), float(alpha), float(eps)
+    a.rows, a.d = x.shape
     if gate is not None:
-        _req(gate.dtype == torch.float32 and gate.is_contiguous() and gate.dim() <= 2 and (gate.dim() < 2 or gate.shape[1] == d), "gate: contiguous fp32 [groups] or [groups, d]")
+        _req(gate.dtype == torch.float32 and gate.dim() <= 2 and (gate.dim() < 2 or gate.shape[1] == a.d), "gate: contiguous fp32 [groups] or [groups, d]")
         a.gate_rows, a.gate_channel = (gate.shape[0] if gate.dim() else 1), int(gate.dim() == 2)
-        _req(a.gate_rows > 0 and rows % a.gate_rows == 0, "gate: %d groups of %d rows" % (a.gate_rows, rows))
-        a.gate = ptr(gate)
+        _req(a.gate_rows > 0 and a.rows % a.gate_rows == 0, "gate: %d groups of %d rows" % (a.gate_rows, a.rows))
     return a
 
 
-def _join_tensors(post, gate, scale, pre):
-    return [*(post or (None, None)), gate, scale, *(pre or (None, None))]
+def _join_call(x, y, post, gate, scale, pre, alpha, eps, rms, gate_tanh):
+    key = ("join", x.dtype, x.shape, y.dtype, y.shape, None if gate is None else (gate.dtype, gate.shape), rms, gate_tanh, alpha, eps)
+    a = L.JoinNormArgs.from_buffer_copy(_plan(key, lambda: _join_plan(x, y, gate, rms, gate_tanh, alpha, eps)))
+    d = a.d
+    if not (x.is_contiguous() and y.is_contiguous() and (gate is None or gate.is_contiguous())):
+        raise L.DeclipHipError("x, y and gate must be contiguous")
+    a.x, a.y = x.data_ptr(), y.data_ptr()
+
+    def vec(t, name):
+        if t.dtype is not torch.float32 or t.numel() != d or not t.is_contiguous():
+            raise L.DeclipHipError("bad argument: %s: contiguous fp32 [%d]" % (name, d))
+        return t.data_ptr()
+
+    for pair, w, b in ((post, "post_w", "post_b"), (pre, "pre_w", "pre_b")):
+        if pair is not None:
+            if pair[0] is None:
+                raise L.DeclipHipError("bad argument: %s: a norm has a weight (a bias alone is none)" % w)
+            setattr(a, w, vec(pair[0], w))
+            if pair[1] is not None:
+                setattr(a, b, vec(pair[1], b))
+    if scale is not None:
+        a.scale = vec(scale, "scale")
+    if gate is not None:
+        a.gate = gate.data_ptr()
+    return a
 
 
 def join_norm_fwd(x, y, *, post=None, gate=None, scale=None, pre=None, alpha=1.0, eps=1e-5, rms=False, gate_tanh=False):
     """A block's boundary in one pass (dh_join_norm_fwd): x_out = alpha x + scale * g * N_post(y), n = N_pre(x_out) -> (x_out, n or None, stats).
     x (residual stream), y (the block's output) [rows, d]; post / pre: (weight, bias or None) fp32 or None (no such norm); gate: fp32 [groups] or [groups, d],
     one value or vector per rows / groups consecutive rows (gate_tanh: tanh of it); scale: fp32 [d]; rms: RMS norms instead of LayerNorms."""
-    with _on_device_of(x, y, *_join_tensors(post, gate, scale, pre)):
-        a = _join_args(x, y, post, gate, scale, pre, alpha, eps, rms, gate_tanh)
-        x_out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        n = torch.empty(x.shape, device=x.device, dtype=x.dtype) if pre is not None else None
-        stats = torch.empty(4, a.rows, device=x.device, dtype=torch.float32)
-        a.x_out, a.n, a.stats = ptr(x_out), ptr(n), ptr(stats)
-        check(L.load().dh_join_norm_fwd(ctypes.byref(a), stream()), "dh_join_norm_fwd")
+    p, n = post or (None, None), pre or (None, None)
+    dev = _device_of(x, y, p[0], p[1], gate, scale, n[0], n[1])
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return join_norm_fwd(x, y, post=post, gate=gate, scale=scale, pre=pre, alpha=alpha, eps=eps, rms=rms, gate_tanh=gate_tanh)
+    a = _join_call(x, y, post, gate, scale, pre, alpha, eps, rms, gate_tanh)
+    x_out, n = torch.empty_like(x), None if pre is None else torch.empty_like(x)
+    stats = torch.empty(4, a.rows, device=x.device, dtype=torch.float32)
+    a.x_out, a.stats = x_out.data_ptr(), stats.data_ptr()
+    if n is not None:
+        a.n = n.data_ptr()
+    check(L.load().dh_join_norm_fwd(ctypes.byref(a), _stream_on(dev)), "dh_join_norm_fwd")
     return x_out, n, stats
 
 
 def join_norm_bwd(x, y, dx_out, dn, stats, *, post=None, gate=None, scale=None, pre=None, alpha=1.0, eps=1e-5, rms=False, gate_tanh=False):
     """Gradients of join_norm_fwd (same arguments, stats: its third result; dx_out or dn may be None) -> (dx, dy, JoinNormGrads); parameter gradients
     are new fp32 tensors of their parameter's shape, None where there is no parameter."""
-    params = _join_tensors(post, gate, scale, pre)
-    with _on_device_of(x, y, dx_out, dn, stats, *params):
-        a = _join_args(x, y, post, gate, scale, pre, alpha, eps, rms, gate_tanh)
-        for t, name in ((dx_out, "dx_out"), (dn, "dn")):
-            _req(t is None or (t.shape == x.shape and t.dtype == x.dtype and t.is_contiguous()), "%s: like x, contiguous" % name)
-        _req(stats.shape == (4, a.rows) and stats.dtype == torch.float32 and stats.is_contiguous(), "stats: the forward's")
-        dx, dy = torch.empty(x.shape, device=x.device, dtype=x.dtype), torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        if a.rows == 0:
-            return dx, dy, JoinNormGrads(*(None if t is None else torch.zeros_like(t) for t in params))
-        grads = JoinNormGrads(*(None if t is None else torch.empty_like(t) for t in params))
-        a.dx_out, a.dn, a.stats, a.dx, a.dy = ptr(dx_out), ptr(dn), ptr(stats), ptr(dx), ptr(dy)
-        a.d_post_w, a.d_post_b, a.d_gate, a.d_scale, a.d_pre_w, a.d_pre_b = (ptr(t) for t in grads)
-        lib = L.load()
-        need = lib.dh_join_norm_bwd_ws_bytes(ctypes.byref(a))
-        ws = torch.empty(max(need, 16) // 4, device=x.device, dtype=torch.float32)
-        a.ws, a.ws_bytes = ptr(ws), need
-        check(lib.dh_join_norm_bwd(ctypes.byref(a), stream()), "dh_join_norm_bwd")
+    p, n = post or (None, None), pre or (None, None)
+    params = (p[0], p[1], gate, scale, n[0], n[1])
+    dev = _device_of(x, y, dx_out, dn, stats, *params)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return join_norm_bwd(x, y, dx_out, dn, stats, post=post, gate=gate, scale=scale, pre=pre, alpha=alpha, eps=eps, rms=rms, gate_tanh=gate_tanh)
+    a = _join_call(x, y, post, gate, scale, pre, alpha, eps, rms, gate_tanh)
+    for t, name in ((dx_out, "dx_out"), (dn, "dn")):
+        if t is not None and not (t.shape == x.shape and t.dtype is x.dtype and t.is_contiguous()):
+            raise L.DeclipHipError("bad argument: %s: like x, contiguous" % name)
+    if stats.shape != (4, a.rows) or stats.dtype is not torch.float32 or not stats.is_contiguous():
+        raise L.DeclipHipError("bad argument: stats: the forward's")
+    dx, dy = torch.empty_like(x), torch.empty_like(x)
+    if a.rows == 0:
+        return dx, dy, JoinNormGrads(*(None if t is None else torch.zeros_like(t) for t in params))
+    grads = JoinNormGrads(*(None if t is None else torch.empty_like(t) for t in params))
+    a.dx_out, a.dn = None if dx_out is None else dx_out.data_ptr(), None if dn is None else dn.data_ptr()
+    a.stats, a.dx, a.dy = stats.data_ptr(), dx.data_ptr(), dy.data_ptr()
+    a.d_post_w, a.d_post_b, a.d_gate, a.d_scale, a.d_pre_w, a.d_pre_b = (None if t is None else t.data_ptr() for t in grads)
+    lib = L.load()
+    need = lib.dh_join_norm_bwd_ws_bytes(ctypes.byref(a))
+    ws = torch.empty(max(need, 16) // 4, device=x.device, dtype=torch.float32)
+    a.ws, a.ws_bytes = ws.data_ptr(), need
+    check(lib.dh_join_norm_bwd(ctypes.byref(a), _stream_on(dev)), "dh_join_norm_bwd")
     return dx, dy, grads

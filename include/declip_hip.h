@@ -232,9 +232,17 @@ int dh_xattn_bwd(const dh_xattn_args* args, dh_stream_t stream);
  *   pair i = columns (i, P + i), interleaved: (2 i, 2 i + 1) of a head
  *   angle  = pos[row % pos_rows][axis] * theta[axis] ^ (-j / sections[axis]), j = the pair's place in its axis (joint: theta ^ (-i / P))
  *   (a, b) -> (a cos - b sin, a sin + b cos); inverse = 1 turns by -angle: the gradient of the rotation
- * pos [pos_rows][axes] int32, or fp32 (pos_float = 1); rows % pos_rows == 0 (a batch of equal grids shares one table).  Angles are formed in 64 bits. */
-int dh_rope_axes(int dtype, const void* x, int64_t ldx, void* y, int64_t ldy, int rows, int heads, int hd, const void* pos, int pos_float,
-                 int pos_rows, const int* sections, const double* theta, int axes, int joint, int interleaved, int inverse, dh_stream_t stream);
+ * pos [pos_rows][axes] int32, or fp32 (pos_float = 1); rows % pos_rows == 0 (a batch of equal grids shares one table).  Angles are formed in 64 bits.
+ * The plan is a host struct: the pairs' frequencies (turns per unit of position) and axes, filled once by dh_rope_plan_init. */
+#define DH_ROPE_MAX_PAIRS 128
+typedef struct {
+  int axes, pairs, hd, interleaved;
+  double turns[DH_ROPE_MAX_PAIRS];
+  unsigned char axis[DH_ROPE_MAX_PAIRS];
+} dh_rope_plan;
+int dh_rope_plan_init(dh_rope_plan* plan, int hd, const int* sections, const double* theta, int axes, int joint, int interleaved);
+int dh_rope_axes(const dh_rope_plan* plan, int dtype, const void* x, int64_t ldx, void* y, int64_t ldy, int rows, int heads, const void* pos,
+                 int pos_float, int pos_rows, int inverse, dh_stream_t stream);
 
 /* ---------------------------------------------------------------- block boundary --------
  * The norm behind a block, its gate and residual scale, the residual sum and the norm in front of the next block in one pass (the residual

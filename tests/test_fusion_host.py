@@ -109,8 +109,8 @@ def test_join_norm_refusals():
         _refused(lambda: f(x, x[:5]), "x and y")
         _refused(lambda: f(x, x.float()), "x and y")
         _refused(lambda: f(x[:, ::2], x[:, ::2]), "contiguous")
-        _refused(lambda: f(x, x, post=(w[:3], None)), "post weight")
-        _refused(lambda: f(x, x, post=(w.to(BF16), None)), "post weight")
+        _refused(lambda: f(x, x, post=(w[:3], None)), "post_w")
+        _refused(lambda: f(x, x, post=(w.to(BF16), None)), "post_w")
         _refused(lambda: f(x, x, post=(w, w), rms=True), "bias")
         _refused(lambda: f(x, x, pre=(None, w)), "bias")
         _refused(lambda: f(x, x, scale=w[:1]), "scale")
@@ -152,9 +152,14 @@ def test_c_entries_check_before_they_launch():
     assert lib.dh_join_norm_fwd(ctypes.byref(j), None) == -1 and b"null output" in lib.dh_last_error()
     assert lib.dh_join_norm_bwd(ctypes.byref(j), None) == -1 and b"workspace" in lib.dh_last_error()
     sec, th = (ctypes.c_int * 1)(4), (ctypes.c_double * 1)(1e4)
-    assert lib.dh_rope_axes(7, one, 64, one, 64, 1, 1, 64, one, 0, 1, sec, th, 1, 0, 0, 0, None) == -1 and b"dtype" in lib.dh_last_error()
-    assert lib.dh_rope_axes(1, one, 32, one, 64, 1, 1, 64, one, 0, 1, sec, th, 1, 0, 0, 0, None) == -1 and b"strides" in lib.dh_last_error()
-    assert lib.dh_rope_axes(1, None, 64, one, 64, 1, 1, 64, one, 0, 1, sec, th, 1, 0, 0, 0, None) == -1
+    plan = L.RopePlan()
+    p = ctypes.byref(plan)
+    assert lib.dh_rope_axes(p, 1, one, 64, one, 64, 2, 1, one, 0, 1, 0, None) == -1 and b"not initialised" in lib.dh_last_error()
+    assert lib.dh_rope_plan_init(None, 64, sec, th, 1, 0, 0) == -1 and lib.dh_rope_plan_init(p, 4, sec, th, 1, 0, 0) == -1 and b"4 pairs in a head of 4" in lib.dh_last_error()
+    assert lib.dh_rope_plan_init(p, 64, sec, th, 1, 0, 0) == 0
+    assert lib.dh_rope_axes(p, 7, one, 64, one, 64, 2, 1, one, 0, 1, 0, None) == -1 and b"dtype" in lib.dh_last_error()
+    assert lib.dh_rope_axes(p, 1, one, 32, one, 64, 2, 1, one, 0, 1, 0, None) == -1 and b"strides" in lib.dh_last_error()
+    assert lib.dh_rope_axes(p, 1, None, 64, one, 64, 2, 1, one, 0, 1, 0, None) == -1
 
 
 def test_cpu_tensors_and_mixed_devices_are_refused():
@@ -171,12 +176,21 @@ def test_a_call_goes_to_its_tensors_device(monkeypatch):
     from declip_amd import ops
     seen = []
 
-    class Dev:
-        type, index = "cuda", 3
+    class Guard:
+        def __init__(self, dev):
+            seen.append(dev)
 
-    class T:
-        is_cuda, device = True, Dev()
+        def __enter__(self):
+            monkeypatch.setattr(torch.cuda, "current_device", lambda: seen[-1])
 
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
-    monkeypatch.setattr(torch.cuda, "device", lambda d: seen.append(d) or "guard")
-    assert ops._on_device_of(T()) == "guard" and seen == [T.device]
+        def __exit__(self, *a):
+            pass
+
+    for call in (lambda x: ops.xattn_fwd(x, x, x, 1, batch=1), lambda x: ops.rope_axes(x, x, 1, (4,)), lambda x: ops.join_norm_fwd(x, x)):
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+        monkeypatch.setattr(torch.cuda, "device", Guard)
+        monkeypatch.setattr(ops, "_device_of", lambda *a: 3)
+        monkeypatch.setattr(ops, "_plan", lambda *a: (_ for _ in ()).throw(RuntimeError("planned on %d" % torch.cuda.current_device())))
+        with pytest.raises(RuntimeError, match="planned on 3"):
+            call(torch.zeros(2, 8))
+    assert seen == [3, 3, 3]
