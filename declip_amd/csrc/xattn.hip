@@ -241,15 +241,16 @@ struct Pair2 {
   static constexpr bool RAGGED = ROWS * NCH % NT != 0;      // fewer tasks than threads, or a last round of fewer
   uint4 a[N], b[N];
   uint8_t keep[N];
-  // pa / pb: bases; off_a / off_b(row): element offsets of a tile row; last: the last row that exists; mask: a byte per row, or NULL
+  // pa / pb: the tile's bases (uniform); off_a / off_b(row): element offsets of its rows from there, 32 bits (scalar base + vector offset, no 64-bit
+  // address per thread); last: the last of its rows that exists; mask: the tile's byte per row, or NULL
   template <typename FA, typename FB>
-  __device__ __forceinline__ void fetch(const T* pa, const T* pb, FA off_a, FB off_b, int first, int last, const uint8_t* mask, int hd, int tid) {
+  __device__ __forceinline__ void fetch(const T* pa, const T* pb, FA off_a, FB off_b, int last, const uint8_t* mask, int hd, int tid) {
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       if (RAGGED && tid + k * NT >= ROWS * NCH) continue;
-      const int task = tid + k * NT, row = min(first + task / NCH, last), c = (task % NCH) * EPC, col = HDP == hd || c < hd ? c : 0;
-      a[k] = *reinterpret_cast<const uint4*>(pa + off_a(row) + col);
-      b[k] = *reinterpret_cast<const uint4*>(pb + off_b(row) + col);
+      const int task = tid + k * NT, row = min(task / NCH, last), c = (task % NCH) * EPC, col = HDP == hd || c < hd ? c : 0;
+      a[k] = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(pa) + (uint32_t)((off_a(row) + col) * (int)sizeof(T)));
+      b[k] = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(pb) + (uint32_t)((off_b(row) + col) * (int)sizeof(T)));
       if (mask) keep[k] = mask[row];
     }
   }
@@ -287,8 +288,10 @@ struct Tiles {
     ldk = p.ldk; ldv = p.ldv; nk = s.nk; hd = p.hd;
   }
   __device__ __forceinline__ void fetch(int kt, int tid) {
-    st.fetch(kb, vb, [&](int r) { return (long)r * ldk; }, [&](int r) { return (long)r * ldv; }, kt * BN, nk - 1, km, hd, tid);
-    if (km && tid < BN) own = km[min(kt * BN + tid, nk - 1)];
+    const int first = kt * BN, last = nk - 1 - first;
+    const uint8_t* m = km ? km + first : nullptr;
+    st.fetch(kb + (long)first * ldk, vb + (long)first * ldv, [&](int r) { return r * (int)ldk; }, [&](int r) { return r * (int)ldv; }, last, m, hd, tid);
+    if (m && tid < BN) own = m[min(tid, last)];
   }
   __device__ __forceinline__ bool edge(int kt) const { return km != nullptr || (kt + 1) * BN > nk; }
   __device__ __forceinline__ void store(int kt, int tid) {
@@ -326,16 +329,52 @@ __device__ __forceinline__ void mask_keys(f32x16_t& sc, const float* bias, int h
   }
 }
 
+// The result rows of a wave leave through LDS as whole rows, 16 bytes per lane (the accumulators hold 4 columns of a row per lane and register group:
+// stored from there a row would be written in 8-byte pieces).  acc[d][4 i + r] = row (lane & 31), column 32 d + 8 i + 4 h + r, times f; row_ptr(r): where
+// row r of the block goes, or nullptr.  U: element type of the result.  Every thread of the block comes here; the LDS is free before and after.
+template <typename U, int HDP, typename F>
+__device__ __forceinline__ void rows_out(unsigned char* smem, const f32x16_t* acc, float f, int hd, int tid, F row_ptr) {
+  constexpr int EPC = Op<U>::EPC, LD = HDP + EPC, DB = HDP / 32, NCH = HDP / EPC;
+  const int lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+  U* mine = reinterpret_cast<U*>(smem) + wave * 32 * LD;
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      Op<U>::store4(mine + (lane & 31) * LD + d * 32 + 8 * i + 4 * h, acc[d][4 * i] * f, acc[d][4 * i + 1] * f, acc[d][4 * i + 2] * f, acc[d][4 * i + 3] * f);
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 32 * NCH / 64; ++k) {
+    const int task = lane + 64 * k, r = task / NCH, c = (task % NCH) * EPC;
+    U* to = row_ptr(wave * 32 + r);
+    if (to && c < hd) *reinterpret_cast<uint4*>(to + c) = *reinterpret_cast<const uint4*>(mine + r * LD + c);
+  }
+  __syncthreads();
+}
+
+// Waves per SIMD a shape is compiled for.  Two (a budget of 256 registers keeps the accumulators out of the accumulation registers, whose moves cost the
+// rescaled forward 192 instructions a tile) unless that spills more than it hides.  Measured in us, 256 captions of 5 .. 77 tokens on 197 keys, 8 heads:
+// hd 128 dq 1 wave per block 87 for one wave per SIMD against 262 for two, dkv of 2 waves per block 180 / 370, of 4 waves 194 / 276; hd 96 (128 sequences
+// of 77) dkv of 4 waves 97 / 79; fp32 hd 64 (16 sequences of 77) dkv 23 / 29, fwd of one wave 17.6 / 23.  RW: waves per block.
+template <typename T, int HDP, int RW> constexpr int waves_fwd() {
+  constexpr int row = HDP * sizeof(T);
+  return RW == 1 ? (row <= 64 ? 3 : sizeof(T) == 2 && row <= 128 ? 2 : 1) : RW == 2 ? (row <= 128 ? 3 : row <= 256 ? 2 : 1) : row <= 384 ? 2 : 1;
+}
+template <typename T, int HDP, int RW> constexpr int waves_dq() {
+  constexpr int row = HDP * sizeof(T);
+  return RW <= 2 && row <= 64 ? 3 : row <= 128 || RW == 8 ? 2 : RW == 1 ? 1 : RW == 2 ? (sizeof(T) == 2 ? 2 : 1) : row <= (sizeof(T) == 2 ? 192 : 256) ? 2 : 1;
+}
+template <typename T, int HDP, int RW> constexpr int waves_dkv() {
+  constexpr int row = HDP * sizeof(T);
+  return RW <= 2 && row <= 64 ? 3 : row <= 128 || RW == 8 || (RW == 4 && row == 192) ? 2 : 1;
+}
+
 // ------------------------------------------------------------------------------------------ forward
-// waves per SIMD to compile for: two where their registers hold everything (a budget of 256 keeps the accumulators out of the accumulation registers, whose
-// moves cost the rescaled forward 192 instructions a tile), else one
-template <typename T, int HDP, int NW> constexpr int waves_fwd() { return NW == 1 ? (HDP * sizeof(T) <= 128 ? 2 : 1) : (HDP * sizeof(T) <= 384 ? 2 : 1); }
-template <typename T, int HDP, int NW, int BN, bool SPLIT>
-__global__ __launch_bounds__(64 * NW, (waves_fwd<T, HDP, NW>())) void xattn_fwd_kernel(XP p) {
-  constexpr int EPC = Op<T>::EPC, LD = HDP + EPC, KS = HDP / (2 * EPC), DB = HDP / 32, NB = BN / 32, BM = 32 * NW, NT = 64 * NW;
+template <typename T, int HDP, int RW, int BN, bool SPLIT>
+__global__ __launch_bounds__(64 * RW, (waves_fwd<T, HDP, RW>())) void xattn_fwd_kernel(XP p) {
+  constexpr int EPC = Op<T>::EPC, LD = HDP + EPC, KS = HDP / (2 * EPC), DB = HDP / 32, NB = BN / 32, BM = 32 * RW, NT = 64 * RW;
   DH_DYN_LDS_A16(unsigned char, smem);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-  const T* q = (const T*)p.q;
   if ((int)blockIdx.x >= p.main_blocks) {
     int first, last;
     owned(p.cu_q, p.batch, p.rows_q, first, last);
@@ -360,11 +399,12 @@ __global__ __launch_bounds__(64 * NW, (waves_fwd<T, HDP, NW>())) void xattn_fwd_
     hi = min(lo + per, nt);
   }
   const float c = p.scale * kLog2e;
+
   for (int t = w.t; (long)t * BM < M; t += p.tiles) {
     const int m = t * BM + wave * 32 + (lane & 31);
     const bool live = m < M, wave_live = t * BM + wave * 32 < M;
     typename Op<T>::Frag qf[KS];
-    load_row<T, HDP>(qf, q + (live ? m_offset(p, s, w.g, m, p.ldq) : 0), live, p.hd, h);
+    load_row<T, HDP>(qf, (const T*)p.q + (live ? m_offset(p, s, w.g, m, p.ldq) : 0), live, p.hd, h);
     f32x16_t o[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -423,61 +463,63 @@ __global__ __launch_bounds__(64 * NW, (waves_fwd<T, HDP, NW>())) void xattn_fwd_
       __syncthreads();                                 // this buffer is read, the other one written
     }
     l += other_half(l);
-    if (live) {
-      const long stat = m_stat(p, s, w.g, m);
-      if (SPLIT) {
-        const long part = (long)w.split * p.heads * p.rows_q + stat;
-        if (h == 0) { p.part_ml[2 * part] = mrun; p.part_ml[2 * part + 1] = l; }
-        if (lo < hi) {
-#pragma unroll
-          for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int col = d * 32 + 8 * i + 4 * h;
-              if (col < p.hd)
-                *reinterpret_cast<float4*>(p.part_o + part * p.hd + col) = make_float4(o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]);
-            }
-        }
-      } else {
-        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-        if (h == 0) p.lse[stat] = l == 0.f ? -INFINITY : (mrun + __log2f(l)) * kLn2;
-        T* orow = (T*)p.out + m_offset(p, s, w.g, m, p.ldo);
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int col = d * 32 + 8 * i + 4 * h;
-            if (col < p.hd) Op<T>::store4(orow + col, o[d][4 * i] * inv, o[d][4 * i + 1] * inv, o[d][4 * i + 2] * inv, o[d][4 * i + 3] * inv);
-          }
-      }
+    const long stat = live ? m_stat(p, s, w.g, m) : 0;
+    if (SPLIT) {
+      const long base = (long)w.split * p.heads * p.rows_q;
+      if (live && h == 0) { p.part_ml[2 * (base + stat)] = mrun; p.part_ml[2 * (base + stat) + 1] = l; }
+      if (lo < hi)
+        rows_out<float, HDP>(smem, o, 1.f, p.hd, tid, [&](int r) -> float* { return t * BM + r < M ? p.part_o + (base + m_stat(p, s, w.g, t * BM + r)) * p.hd : nullptr; });
+    } else {
+      if (live && h == 0) p.lse[stat] = l == 0.f ? -INFINITY : (mrun + __log2f(l)) * kLn2;
+      rows_out<T, HDP>(smem, o, l == 0.f ? 0.f : 1.f / l, p.hd, tid,
+                       [&](int r) -> T* { return t * BM + r < M ? (T*)p.out + m_offset(p, s, w.g, t * BM + r, p.ldo) : nullptr; });
     }
   }
 }
 
-// joins the key ranges of one (query row, head): o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, ranges in ascending order.  A wave per pair: its lanes
-// read the ranges' (m, l) at once, and a lane's columns of the partial sums are independent loads.
-template <typename T>
+// joins the key ranges of one (query row, head): o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, in a fixed order.  JW waves per pair (4: many ranges, few
+// pairs) take every JW-th range; their lanes read the ranges' (m, l) at once, and a lane's columns of eight partial sums are independent loads.
+template <typename T, int JW>
 __global__ __launch_bounds__(256) void xattn_join_kernel(XP p) {
+  __shared__ float2 part_sum[4][64];
   int first = 0, last = p.rows_q;
   if (p.cu_q) owned(p.cu_q, p.batch, p.rows_q, first, last);
-  const int lane = threadIdx.x & 63, c0 = 2 * lane;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c0 = 2 * lane, w = JW == 1 ? 0 : wave;
   const long n = (long)(last - first) * p.heads, stride = (long)p.heads * p.rows_q;
-  for (long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += (long)gridDim.x * 4) {
+  for (long i0 = (long)blockIdx.x * (4 / JW); i0 < n; i0 += (long)gridDim.x * (4 / JW)) {
+    const long i = i0 + (JW == 1 ? wave : 0);
+    if (JW == 1 && i >= n) break;
     const int row = first + (int)(i / p.heads), head = (int)(i % p.heads);
     const long stat = (long)head * p.rows_q + row;
     float2 ml = make_float2(-INFINITY, 0.f);
     if (lane < p.nsplit) ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * (lane * stride + stat));
     const float m = wave_max(ml.x), f = ml.y == 0.f ? 0.f : exp2_fast(ml.x - m), l = wave_sum(f * ml.y);
     float2 acc = make_float2(0.f, 0.f);
-    const float* part = p.part_o + stat * p.hd + c0;
-#pragma unroll 4
-    for (int s = 0; s < p.nsplit; ++s) {
-      const float fs = __shfl(f, s, 64);
-      if (fs != 0.f && c0 < p.hd) {                  // (an empty range wrote no sums)
-        const float2 v = *reinterpret_cast<const float2*>(part + s * stride * p.hd);
-        acc.x = fmaf(fs, v.x, acc.x);
-        acc.y = fmaf(fs, v.y, acc.y);
+    const float* part = p.part_o + stat * p.hd + (c0 < p.hd ? c0 : 0);
+    for (int s0 = w; s0 < p.nsplit; s0 += 8 * JW) {
+      float2 v[8];
+      float fs[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int s = min(s0 + k * JW, p.nsplit - 1);
+        v[k] = *reinterpret_cast<const float2*>(part + s * stride * p.hd);
+        fs[k] = s0 + k * JW < p.nsplit ? __shfl(f, s, 64) : 0.f;
       }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (fs[k] != 0.f) {                          // (an empty range wrote no sums)
+          acc.x = fmaf(fs[k], v[k].x, acc.x);
+          acc.y = fmaf(fs[k], v[k].y, acc.y);
+        }
+    }
+    if (JW > 1) {
+      __syncthreads();
+      part_sum[wave][lane] = acc;
+      __syncthreads();
+      if (wave) continue;
+      acc = part_sum[0][lane];
+#pragma unroll
+      for (int k = 1; k < JW; ++k) { acc.x += part_sum[k][lane].x; acc.y += part_sum[k][lane].y; }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     T* o = (T*)p.out + (long)row * p.ldo + (long)head * p.hd + c0;
@@ -486,10 +528,31 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XP p) {
   }
 }
 
+// gradients whose other axis was split: the ranges' sums added in ascending order, times f.  part [nsplit][rows][width] fp32 -> out [rows][width]
+template <typename T>
+__global__ __launch_bounds__(256) void xattn_sum_kernel(const float* part, T* out, long ldo, int rows, int width, int nsplit, float f, const int* cu, int batch) {
+  int first = 0, last = rows;
+  if (cu) owned(cu, batch, rows, first, last);
+  const int nch = width / 4;
+  const long n = (long)(last - first) * nch, stride = (long)rows * width;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
+    const long row = first + i / nch;
+    const int c = (int)(i % nch) * 4;
+    const float* x = part + row * width + c;
+    float4 s = *reinterpret_cast<const float4*>(x);
+#pragma unroll 4
+    for (int k = 1; k < nsplit; ++k) {
+      const float4 v = *reinterpret_cast<const float4*>(x + k * stride);
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    Op<T>::store4(out + row * ldo + c, s.x * f, s.y * f, s.z * f, s.w * f);
+  }
+}
+
 // ------------------------------------------------------------------------------------------ backward: dq (and D)
-template <typename T, int HDP, int NW, int BN>
-__global__ __launch_bounds__(64 * NW, NW == 8 || HDP <= 64 ? 2 : 1) void xattn_dq_kernel(XP p) {
-  constexpr int EPC = Op<T>::EPC, LD = HDP + EPC, KS = HDP / (2 * EPC), DB = HDP / 32, NB = BN / 32, BM = 32 * NW, NT = 64 * NW;
+template <typename T, int HDP, int RW, int BN, bool SPLIT>
+__global__ __launch_bounds__(64 * RW, (waves_dq<T, HDP, RW>())) void xattn_dq_kernel(XP p) {
+  constexpr int EPC = Op<T>::EPC, LD = HDP + EPC, KS = HDP / (2 * EPC), DB = HDP / 32, NB = BN / 32, BM = 32 * RW, NT = 64 * RW;
   DH_DYN_LDS_A16(unsigned char, smem);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
   if ((int)blockIdx.x >= p.main_blocks) {
@@ -502,6 +565,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || HDP <= 64 ? 2 : 1) void xattn_d
   if (!w.live) return;
   const Seq s = seq_of(p, w.b);
   const int M = s.nq * p.rep, nt = (s.nk + BN - 1) / BN;
+  const int per = SPLIT ? (nt + p.nsplit - 1) / p.nsplit : nt, lo = SPLIT ? min(w.split * per, nt) : 0, hi = SPLIT ? min(lo + per, nt) : nt;   // this block's key tiles
   const float c = p.scale * kLog2e;
   for (int t = w.t; (long)t * BM < M; t += p.tiles) {
     const int m = t * BM + wave * 32 + (lane & 31);
@@ -521,30 +585,31 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || HDP <= 64 ? 2 : 1) void xattn_d
       for (int ks = 0; ks < KS; ++ks) D += Op<T>::dot(df[ks], of[ks]);
     }
     D += other_half(D);
-    if (live && h == 0) p.delta[stat] = D;
+    if (live && h == 0 && (!SPLIT || w.split == 0)) p.delta[stat] = D;
     f32x16_t dq[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) dq[d][i] = 0.f;
     Tiles<T, HDP, BN, NT> kt_(p, s, w.g, smem);
-    kt_.begin(0, nt, tid);
-    for (int kt = 0; kt < nt; ++kt) {
+    kt_.begin(lo, hi, tid);
+    for (int kt = lo; kt < hi; ++kt) {
       const T *Ks, *Vs;
       const float* bias;
-      const bool masked = kt_.next(kt, nt, tid, Ks, Vs, bias);
-      if (wave_live) {
-        auto p_dp = [&](int b, f32x16_t& sc, f32x16_t& dp) {     // p and dp of 32 keys
-          sc = mma_row<T, HDP>(Ks, LD, b * 32, qf, lane);
-          dp = mma_row<T, HDP>(Vs, LD, b * 32, df, lane);
-          if (masked) mask_keys(sc, bias + b * 32, h);
+      const bool masked = kt_.next(kt, hi, tid, Ks, Vs, bias);
+      const bool busy = wave_live;
+      auto p_dp = [&](int b, f32x16_t& sc, f32x16_t& dp) {     // p and dp of 32 keys
+        sc = mma_row<T, HDP>(Ks, LD, b * 32, qf, lane);
+        dp = mma_row<T, HDP>(Vs, LD, b * 32, df, lane);
+        if (masked) mask_keys(sc, bias + b * 32, h);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sc[i] = exp2_fast(fmaf(sc[i], c, -lse2));
-        };
-        if (sizeof(T) == 2 && nt == 1) {
-          // all keys are here: D = sum p dp, which is sum(do o) before o was rounded.  With a few keys dp - D cancels, and the rounding of o
-          // alone would double the error of dq and dk (two keys: 3.6e-3 instead of 2.4e-3 of their norm); over many keys |o| is small against |v|.
-          D = 0.f;
+        for (int i = 0; i < 16; ++i) sc[i] = exp2_fast(fmaf(sc[i], c, -lse2));
+      };
+      if (sizeof(T) == 2 && nt == 1) {
+        // all keys are here: D = sum p dp, which is sum(do o) before o was rounded.  With a few keys dp - D cancels, and the rounding of o
+        // alone would double the error of dq and dk (two keys: 3.6e-3 instead of 2.4e-3 of their norm); over many keys |o| is small against |v|.
+        D = 0.f;
+        if (busy) {
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
             f32x16_t sc, dp;
@@ -552,9 +617,11 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || HDP <= 64 ? 2 : 1) void xattn_d
 #pragma unroll
             for (int i = 0; i < 16; ++i) D = fmaf(sc[i], dp[i], D);
           }
-          D += other_half(D);
-          if (live && h == 0) p.delta[stat] = D;
         }
+        D += other_half(D);
+        if (live && h == 0 && (!SPLIT || w.split == 0)) p.delta[stat] = D;
+      }
+      if (busy) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
           f32x16_t sc, dp;
@@ -568,23 +635,19 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || HDP <= 64 ? 2 : 1) void xattn_d
       }
       __syncthreads();
     }
-    if (live) {
-      T* row = (T*)p.dq + m_offset(p, s, w.g, m, p.lddq);
-#pragma unroll
-      for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int col = d * 32 + 8 * i + 4 * h;
-          if (col < p.hd) Op<T>::store4(row + col, dq[d][4 * i] * p.scale, dq[d][4 * i + 1] * p.scale, dq[d][4 * i + 2] * p.scale, dq[d][4 * i + 3] * p.scale);
-        }
+    if (SPLIT) {
+      float* part = p.part_o + (long)w.split * p.rows_q * p.heads * p.hd;
+      rows_out<float, HDP>(smem, dq, 1.f, p.hd, tid, [&](int r) -> float* { return t * BM + r < M ? part + m_offset(p, s, w.g, t * BM + r, (long)p.heads * p.hd) : nullptr; });
+    } else {
+      rows_out<T, HDP>(smem, dq, p.scale, p.hd, tid, [&](int r) -> T* { return t * BM + r < M ? (T*)p.dq + m_offset(p, s, w.g, t * BM + r, p.lddq) : nullptr; });
     }
   }
 }
 
 // ------------------------------------------------------------------------------------------ backward: dk, dv
-template <typename T, int HDP, int NW, int BQ>
-__global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(T) * HDP <= 128 ? 2 : 1) void xattn_dkv_kernel(XP p) {
-  constexpr int EPC = Op<T>::EPC, LD = HDP + EPC, KS = HDP / (2 * EPC), DB = HDP / 32, NB = BQ / 32, BK = 32 * NW, NT = 64 * NW;
+template <typename T, int HDP, int RW, bool SPLIT>
+__global__ __launch_bounds__(64 * RW, (waves_dkv<T, HDP, RW>())) void xattn_dkv_kernel(XP p) {
+  constexpr int EPC = Op<T>::EPC, LD = HDP + EPC, KS = HDP / (2 * EPC), DB = HDP / 32, BQ = 32, BK = 32 * RW, NT = 64 * RW;
   DH_DYN_LDS_A16(unsigned char, smem);
   T* buf = reinterpret_cast<T*>(smem);                 // two buffers of Q and dO rows, lse and D of the rows
   float* stats = reinterpret_cast<float*>(buf + 4 * BQ * LD);
@@ -601,10 +664,11 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(T) * HDP <= 128 ? 2 : 1)
   if (!w.live) return;
   const Seq s = seq_of(p, w.b);
   const int M = s.nq * p.rep, nt = (M + BQ - 1) / BQ;
+  const int per = SPLIT ? (nt + p.nsplit - 1) / p.nsplit : nt, lo = SPLIT ? min(w.split * per, nt) : 0, hi = SPLIT ? min(lo + per, nt) : nt;   // this block's row tiles
   const float c = p.scale * kLog2e;
   for (int t = w.t; (long)t * BK < s.nseg; t += p.tiles) {
     const int key = t * BK + wave * 32 + (lane & 31);
-    const bool in = key < s.nseg, live = key < s.nk && (!p.key_mask || p.key_mask[s.k0 + key]);
+    const bool live = key < s.nk && (!p.key_mask || p.key_mask[s.k0 + key]);
     const bool wave_live = t * BK + wave * 32 < s.nk, block_live = t * BK < s.nk;
     typename Op<T>::Frag kf[KS], vf[KS];
     load_row<T, HDP>(kf, (const T*)p.k + (live ? (long)(s.k0 + key) * p.ldk + (long)w.g * p.hd : 0), live, p.hd, h);
@@ -617,8 +681,12 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(T) * HDP <= 128 ? 2 : 1)
     Pair2<T, HDP, BQ, NT> st;
     float nlse = 0.f, ndel = 0.f;
     auto fetch = [&](int mt) {
-      st.fetch((const T*)p.q, (const T*)p.dout, [&](int m) { return m_offset(p, s, w.g, m, p.ldq); }, [&](int m) { return m_offset(p, s, w.g, m, p.lddo); },
-               mt * BQ, M - 1, nullptr, p.hd, tid);
+      const int m0 = mt * BQ;
+      int q0, r0;
+      m_split(p, m0, q0, r0);                          // (uniform: the tile's first row)
+      auto off = [&](int r, long ld) { int q, x; m_split(p, m0 + r, q, x); return (q - q0) * (int)ld + x * p.hd; };
+      st.fetch((const T*)p.q + (long)(s.q0 + q0) * p.ldq + (long)w.g * p.rep * p.hd, (const T*)p.dout + (long)(s.q0 + q0) * p.lddo + (long)w.g * p.rep * p.hd,
+               [&](int r) { return off(r, p.ldq); }, [&](int r) { return off(r, p.lddo); }, M - 1 - m0, nullptr, p.hd, tid);
       if (tid < BQ) {
         const long stat = m_stat(p, s, w.g, min(mt * BQ + tid, M - 1));
         nlse = p.lse[stat];
@@ -634,60 +702,57 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(T) * HDP <= 128 ? 2 : 1)
         x[BQ] = ndel;
       }
     };
-    const int n_mt = block_live ? nt : 0;
-    if (n_mt > 0) {
-      fetch(0);
-      store(0);
-      if (n_mt > 1) fetch(1);
+    const int hi_mt = block_live ? hi : lo;
+    if (lo < hi_mt) {
+      fetch(lo);
+      store(lo);
+      if (lo + 1 < hi_mt) fetch(lo + 1);
       __syncthreads();
     }
-    for (int mt = 0; mt < n_mt; ++mt) {
-      if (mt + 1 < n_mt) {
+    for (int mt = lo; mt < hi_mt; ++mt) {
+      if (mt + 1 < hi_mt) {
         store(mt + 1);
-        if (mt + 2 < n_mt) fetch(mt + 2);
+        if (mt + 2 < hi_mt) fetch(mt + 2);
       }
       if (wave_live) {
         const T *Qs = buf + (mt & 1) * 2 * BQ * LD, *Ds = Qs + BQ * LD;
         const float *lse2s = stats + (mt & 1) * 2 * BQ, *dels = lse2s + BQ;
+        f32x16_t sc = mma_row<T, HDP>(Qs, LD, 0, kf, lane);
+        f32x16_t dp = mma_row<T, HDP>(Ds, LD, 0, vf, lane);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          f32x16_t sc = mma_row<T, HDP>(Qs, LD, b * 32, kf, lane);
-          f32x16_t dp = mma_row<T, HDP>(Ds, LD, b * 32, vf, lane);
+        for (int i = 0; i < 4; ++i) {
+          const float4 L = *reinterpret_cast<const float4*>(lse2s + 8 * i + 4 * h);
+          const float4 D = *reinterpret_cast<const float4*>(dels + 8 * i + 4 * h);
+          sc[4 * i] = exp2_fast(fmaf(sc[4 * i], c, -L.x)); dp[4 * i] = sc[4 * i] * (dp[4 * i] - D.x);
+          sc[4 * i + 1] = exp2_fast(fmaf(sc[4 * i + 1], c, -L.y)); dp[4 * i + 1] = sc[4 * i + 1] * (dp[4 * i + 1] - D.y);
+          sc[4 * i + 2] = exp2_fast(fmaf(sc[4 * i + 2], c, -L.z)); dp[4 * i + 2] = sc[4 * i + 2] * (dp[4 * i + 2] - D.z);
+          sc[4 * i + 3] = exp2_fast(fmaf(sc[4 * i + 3], c, -L.w)); dp[4 * i + 3] = sc[4 * i + 3] * (dp[4 * i + 3] - D.w);
+        }
+        const typename Op<T>::PF pf = Op<T>::pack(sc), sf = Op<T>::pack(dp);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float4 L = *reinterpret_cast<const float4*>(lse2s + b * 32 + 8 * i + 4 * h);
-            const float4 D = *reinterpret_cast<const float4*>(dels + b * 32 + 8 * i + 4 * h);
-            sc[4 * i] = exp2_fast(fmaf(sc[4 * i], c, -L.x)); dp[4 * i] = sc[4 * i] * (dp[4 * i] - D.x);
-            sc[4 * i + 1] = exp2_fast(fmaf(sc[4 * i + 1], c, -L.y)); dp[4 * i + 1] = sc[4 * i + 1] * (dp[4 * i + 1] - D.y);
-            sc[4 * i + 2] = exp2_fast(fmaf(sc[4 * i + 2], c, -L.z)); dp[4 * i + 2] = sc[4 * i + 2] * (dp[4 * i + 2] - D.z);
-            sc[4 * i + 3] = exp2_fast(fmaf(sc[4 * i + 3], c, -L.w)); dp[4 * i + 3] = sc[4 * i + 3] * (dp[4 * i + 3] - D.w);
-          }
-          const typename Op<T>::PF pf = Op<T>::pack(sc), sf = Op<T>::pack(dp);
-#pragma unroll
-          for (int d = 0; d < DB; ++d) {
-            Op<T>::mma_t(dv[d], Ds, LD, b * 32, d * 32, pf, lane);
-            Op<T>::mma_t(dk[d], Qs, LD, b * 32, d * 32, sf, lane);
-          }
+        for (int d = 0; d < DB; ++d) {
+          Op<T>::mma_t(dv[d], Ds, LD, 0, d * 32, pf, lane);
+          Op<T>::mma_t(dk[d], Qs, LD, 0, d * 32, sf, lane);
         }
       }
       __syncthreads();
     }
-    if (in) {
-      T* krow = (T*)p.dk + (long)(s.k0 + key) * p.lddk + (long)w.g * p.hd;
-      T* vrow = (T*)p.dv + (long)(s.k0 + key) * p.lddv + (long)w.g * p.hd;
-      // (a masked key's column may hold anything: it is written as zeros)
+    // (a masked key's column may hold anything: it is written as zeros)
+    if (!live)
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int col = d * 32 + 8 * i + 4 * h;
-          if (col >= p.hd) continue;
-          float a[4], b[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) { a[r] = live ? dk[d][4 * i + r] * p.scale : 0.f; b[r] = live ? dv[d][4 * i + r] : 0.f; }
-          Op<T>::store4(krow + col, a[0], a[1], a[2], a[3]);
-          Op<T>::store4(vrow + col, b[0], b[1], b[2], b[3]);
-        }
+        for (int i = 0; i < 16; ++i) dk[d][i] = dv[d][i] = 0.f;
+    if (SPLIT) {
+      const long width = (long)p.kv_heads * p.hd, all = (long)p.rows_kv * width;
+      float* part = p.part_o + (long)w.split * all;
+      auto row = [&](float* x, int r) -> float* { return t * BK + r < s.nseg ? x + (long)(s.k0 + t * BK + r) * width + (long)w.g * p.hd : nullptr; };
+      rows_out<float, HDP>(smem, dk, 1.f, p.hd, tid, [&](int r) { return row(part, r); });
+      rows_out<float, HDP>(smem, dv, 1.f, p.hd, tid, [&](int r) { return row(part + p.nsplit * all, r); });
+    } else {
+      auto row = [&](T* x, long ld, int r) -> T* { return t * BK + r < s.nseg ? x + (long)(s.k0 + t * BK + r) * ld + (long)w.g * p.hd : nullptr; };
+      rows_out<T, HDP>(smem, dk, p.scale, p.hd, tid, [&](int r) { return row((T*)p.dk, p.lddk, r); });
+      rows_out<T, HDP>(smem, dv, 1.f, p.hd, tid, [&](int r) { return row((T*)p.dv, p.lddv, r); });
     }
   }
 }
@@ -704,6 +769,7 @@ int x_cus() {
 }
 
 int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int64_t round4(int64_t n) { return (n + 3) & ~(int64_t)3; }
 
 // longest length to lay the grid out for: the caller's bound, or twice the mean of a packed batch (longer ones take several rounds)
 int length_hint(int given, const int* cu, int rows, int batch) {
@@ -712,27 +778,44 @@ int length_hint(int given, const int* cu, int rows, int batch) {
   return (int)(n > rows ? rows : n);
 }
 
-// heads of more than 64 columns, bf16, many rows: 8 waves share a tile (half the staging registers each, so two waves fit a SIMD)
-bool wide_block(const dh_xattn_args* a, int64_t mq) { return a->dtype == DH_BF16 && a->hd > 64 && mq > 128; }
-struct Plan { int nw, bn, tiles, nsplit; };
-Plan plan_fwd(const dh_xattn_args* a) {
-  const int rep = a->heads / a->kv_heads;
-  const int64_t mq = (int64_t)length_hint(a->max_q, a->cu_q, a->rows_q, a->batch) * rep;
-  const int mk = length_hint(a->max_kv, a->cu_kv, a->rows_kv, a->batch);
+enum Kind { FWD, DQ, DKV };
+// Waves of 32 rows per block; they share the tiles of the other axis.  Long axes want many (less staging per row), short ones few: blocks of one wave
+// wait for nobody and more sequences are under way at a time.  Measured in us (bf16, one / two / four waves): 2048 (sequence, head) pairs of 5 .. 77 rows
+// on 197 keys fwd 31 / 39 / 42, dq 36 / 52 / 48, dkv 58 / 60 / 62; 197 rows on 5 .. 77 keys fwd 42 / 37 / 48, dq 58 / 65 / 72; 128 pairs of 512 on 512 fwd
+// 26 / 23 / 18, dkv 39 / 32 / 29; 24 pairs of 2047 on 6272 fwd 226 / 198 / 147.
+// More than 64 columns: eight waves (half of the staging registers each, two waves per SIMD) once they are filled: 16 pairs of 4096 rows on 3136 keys fwd
+// 164 (four: 170), dq 191 (319), dkv 382 (612).  fp32 is bound by its matrix instructions: four.
+int row_waves(const dh_xattn_args* a, Kind kind, int64_t rows, int64_t other) {
+  if (rows <= 32) return 1;
+  if (a->dtype == DH_F32) return 4;
+  if (a->hd <= 64) return rows <= 128 || other <= 256 ? 1 : 4;
+  if (kind == DKV && a->hd > 96 && other <= 128) return 2;
+  if (rows > 128) return 8;
+  return kind == DQ ? 1 : 4;
+}
+// A launch over (sequence, kv head) pairs: `rows` of one axis in tiles of rw 32; the other axis (`other` long) split in ranges of at least `step` where
+// the tiles alone leave compute units idle.
+struct Plan { int rw, tiles, nsplit; };
+Plan plan_of(const dh_xattn_args* a, Kind kind, int64_t rows, int64_t other, int step) {
   Plan r;
-  r.nw = mq <= 32 ? 1 : wide_block(a, mq) ? 8 : 4;
-  r.bn = (r.nw == 1 || a->dtype == DH_F32) ? 32 : 64;
-  r.tiles = (int)cdiv64(mq < 1 ? 1 : mq, 32 * r.nw);
-  const int64_t blocks = (int64_t)r.tiles * a->batch * a->kv_heads, want = (int64_t)x_cus() * (8 / r.nw);
+  r.rw = row_waves(a, kind, rows, other);
+  r.tiles = (int)cdiv64(rows < 1 ? 1 : rows, 32 * r.rw);
+  const int64_t blocks = (int64_t)r.tiles * a->batch * a->kv_heads, want = (int64_t)x_cus() * (8 / r.rw);
   int64_t ns = blocks >= want ? 1 : want / blocks;
-  const int64_t most = cdiv64(mk, 4 * r.bn);          // a range is at least four tiles long
+  const int64_t most = cdiv64(other, step);
   if (ns > most) ns = most;
   if (ns > 64) ns = 64;
   r.nsplit = ns < 1 ? 1 : (int)ns;
   return r;
 }
+int64_t longest_m(const dh_xattn_args* a) { return (int64_t)length_hint(a->max_q, a->cu_q, a->rows_q, a->batch) * (a->heads / a->kv_heads); }
+int longest_k(const dh_xattn_args* a) { return length_hint(a->max_kv, a->cu_kv, a->rows_kv, a->batch); }
+// forward and dq split the keys, dkv the query rows; a range is at least 128 (fwd) / 256 long: its partial result costs as much as a few tiles
+Plan plan_fwd(const dh_xattn_args* a) { return plan_of(a, FWD, longest_m(a), longest_k(a), 128); }
+Plan plan_dq(const dh_xattn_args* a) { return plan_of(a, DQ, longest_m(a), longest_k(a), 256); }
+Plan plan_dkv(const dh_xattn_args* a) { return plan_of(a, DKV, longest_k(a), longest_m(a), 256); }
 
-int check_args(const dh_xattn_args* a, const char* who, bool bwd) {
+int check_geometry(const dh_xattn_args* a, const char* who) {
   DH_REQUIRE(a, "%s: null args", who);
   DH_REQUIRE(a->dtype == DH_F32 || a->dtype == DH_BF16, "%s: dtype %d", who, a->dtype);
   DH_REQUIRE(a->batch > 0 && a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0, "%s: batch %d, heads %d, kv_heads %d", who, a->batch, a->heads, a->kv_heads);
@@ -742,6 +825,10 @@ int check_args(const dh_xattn_args* a, const char* who, bool bwd) {
   DH_REQUIRE(a->cu_kv || a->rows_kv % a->batch == 0, "%s: %d key rows do not divide into %d sequences", who, a->rows_kv, a->batch);
   DH_REQUIRE(a->scale > 0.f && a->scale < INFINITY, "%s: scale must be positive and finite", who);
   DH_REQUIRE((int64_t)a->rows_q * (a->heads / a->kv_heads) < (1ll << 30) && a->rows_kv < (1 << 30), "%s: too many rows", who);
+  return DH_OK;
+}
+int check_args(const dh_xattn_args* a, const char* who, bool bwd) {
+  if (int e = check_geometry(a, who)) return e;
   const int epc = a->dtype == DH_BF16 ? 8 : 4;
   const int64_t wq = (int64_t)a->heads * a->hd, wk = (int64_t)a->kv_heads * a->hd;
   struct { const void* p; int64_t ld, w; bool need; const char* name; } m[] = {
@@ -751,7 +838,7 @@ int check_args(const dh_xattn_args* a, const char* who, bool bwd) {
   for (const auto& x : m) {
     if (!x.need) continue;
     DH_REQUIRE(x.p, "%s: %s is NULL", who, x.name);
-    DH_REQUIRE(((uintptr_t)x.p & 15) == 0 && x.ld >= x.w && x.ld % epc == 0, "%s: %s needs 16-byte aligned rows (row stride %lld, width %lld)", who, x.name,
+    DH_REQUIRE(((uintptr_t)x.p & 15) == 0 && x.ld >= x.w && x.ld % epc == 0 && x.ld < (1 << 22), "%s: %s needs 16-byte aligned rows, row strides up to 2^22 (row stride %lld, width %lld)", who, x.name,
                (long long)x.ld, (long long)x.w);
   }
   DH_REQUIRE(a->lse || a->rows_q == 0, "%s: lse is NULL", who);
@@ -792,57 +879,114 @@ int launch(K kernel, const XP& p, int64_t grid, int threads, size_t lds, hipStre
   return DH_OK;
 }
 
-// two buffers of two tiles, `per_row` floats beside each tile row
-template <typename T, int HDP> constexpr size_t tile_bytes(int rows, int per_row) { return 2 * ((size_t)2 * rows * (HDP + Op<T>::EPC) * sizeof(T) + (size_t)rows * per_row * 4); }
+// LDS of a block: two buffers of two tiles with `per_row` floats beside each tile row; the result rows go through it at the end (fp32 where split)
+template <typename T, int HDP, int RW> constexpr size_t lds_bytes(int rows, int per_row, bool split) {
+  const size_t tiles = 2 * ((size_t)2 * rows * (HDP + Op<T>::EPC) * sizeof(T) + (size_t)rows * per_row * 4);
+  const size_t out = split || sizeof(T) == 4 ? (size_t)RW * 32 * (HDP + 4) * 4 : (size_t)RW * 32 * (HDP + Op<T>::EPC) * sizeof(T);
+  return tiles > out ? tiles : out;
+}
+template <typename T, int HDP, int RW, int BN>
+int fwd_shape(XP& p, int64_t grid, hipStream_t st) {
+  static_assert(lds_bytes<T, HDP, RW>(BN, 1, true) <= 160 * 1024, "LDS");
+  const size_t lds = lds_bytes<T, HDP, RW>(BN, 1, p.nsplit > 1);
+  return p.nsplit > 1 ? launch(xattn_fwd_kernel<T, HDP, RW, BN, true>, p, grid, 64 * RW, lds, st) : launch(xattn_fwd_kernel<T, HDP, RW, BN, false>, p, grid, 64 * RW, lds, st);
+}
+template <typename T, int HDP, int RW, int BN>
+int dq_shape(XP& p, int64_t grid, hipStream_t st) {
+  const size_t lds = lds_bytes<T, HDP, RW>(BN, 1, p.nsplit > 1);
+  return p.nsplit > 1 ? launch(xattn_dq_kernel<T, HDP, RW, BN, true>, p, grid, 64 * RW, lds, st) : launch(xattn_dq_kernel<T, HDP, RW, BN, false>, p, grid, 64 * RW, lds, st);
+}
+template <typename T, int HDP, int RW>
+int dkv_shape(XP& p, int64_t grid, hipStream_t st) {
+  const size_t lds = lds_bytes<T, HDP, RW>(32, 2, p.nsplit > 1);
+  return p.nsplit > 1 ? launch(xattn_dkv_kernel<T, HDP, RW, true>, p, grid, 64 * RW, lds, st) : launch(xattn_dkv_kernel<T, HDP, RW, false>, p, grid, 64 * RW, lds, st);
+}
 
 template <typename T, int HDP>
-int fwd_hd(XP& p, const Plan& pl, int64_t grid, hipStream_t st) {
+int fwd_hd(XP& p, int rw, int64_t grid, hipStream_t st) {
   constexpr int BN = sizeof(T) == 2 ? 64 : 32;
-  const size_t lds1 = tile_bytes<T, HDP>(32, 1), lds4 = tile_bytes<T, HDP>(BN, 1);
-  if (pl.nw == 1) return pl.nsplit > 1 ? launch(xattn_fwd_kernel<T, HDP, 1, 32, true>, p, grid, 64, lds1, st) : launch(xattn_fwd_kernel<T, HDP, 1, 32, false>, p, grid, 64, lds1, st);
-  if constexpr (sizeof(T) == 2 && HDP > 64) {
-    if (pl.nw == 8) return pl.nsplit > 1 ? launch(xattn_fwd_kernel<T, HDP, 8, BN, true>, p, grid, 512, lds4, st) : launch(xattn_fwd_kernel<T, HDP, 8, BN, false>, p, grid, 512, lds4, st);
-  }
-  return pl.nsplit > 1 ? launch(xattn_fwd_kernel<T, HDP, 4, BN, true>, p, grid, 256, lds4, st) : launch(xattn_fwd_kernel<T, HDP, 4, BN, false>, p, grid, 256, lds4, st);
+  if constexpr (sizeof(T) == 2 && HDP > 64)
+    if (rw == 8) return fwd_shape<T, HDP, 8, BN>(p, grid, st);
+  return rw == 1 ? fwd_shape<T, HDP, 1, 32>(p, grid, st) : rw == 2 ? fwd_shape<T, HDP, 2, 32>(p, grid, st) : fwd_shape<T, HDP, 4, BN>(p, grid, st);
 }
 template <typename T, int HDP>
-int bwd_hd(XP& p, const dh_xattn_args* a, hipStream_t st) {
+int dq_hd(XP& p, int rw, int64_t grid, hipStream_t st) {
   constexpr int BN = sizeof(T) == 2 ? 64 : 32;
-  int64_t grid;
-  const int64_t mq = (int64_t)length_hint(a->max_q, a->cu_q, a->rows_q, a->batch) * p.rep;
-  if (a->rows_q > 0) {
-    const bool wide = wide_block(a, mq);
-    if (int e = lay_out(p, (int)cdiv64(mq, wide ? 256 : 128), 1, a->cu_q != nullptr, grid)) return e;
-    if constexpr (sizeof(T) == 2 && HDP > 64) {
-      if (wide)
-        if (int e = launch(xattn_dq_kernel<T, HDP, 8, BN>, p, grid, 512, tile_bytes<T, HDP>(BN, 1), st)) return e;
-    }
-    if (!wide)
-      if (int e = launch(xattn_dq_kernel<T, HDP, 4, BN>, p, grid, 256, tile_bytes<T, HDP>(BN, 1), st)) return e;
-  }
-  if (a->rows_kv > 0) {
-    const int mk = length_hint(a->max_kv, a->cu_kv, a->rows_kv, a->batch);
-    const bool wide = a->dtype == DH_BF16 && a->hd > 64 && mk > 128;
-    if (int e = lay_out(p, (int)cdiv64(mk, wide ? 256 : 128), 1, a->cu_kv != nullptr, grid)) return e;
-    if constexpr (sizeof(T) == 2 && HDP > 64) {
-      if (wide) return launch(xattn_dkv_kernel<T, HDP, 8, 32>, p, grid, 512, tile_bytes<T, HDP>(32, 2), st);
-    }
-    return launch(xattn_dkv_kernel<T, HDP, 4, 32>, p, grid, 256, tile_bytes<T, HDP>(32, 2), st);
-  }
+  if constexpr (sizeof(T) == 2 && HDP > 64)
+    if (rw == 8) return dq_shape<T, HDP, 8, BN>(p, grid, st);
+  return rw == 1 ? dq_shape<T, HDP, 1, 32>(p, grid, st) : rw == 2 ? dq_shape<T, HDP, 2, 32>(p, grid, st) : dq_shape<T, HDP, 4, BN>(p, grid, st);
+}
+template <typename T, int HDP>
+int dkv_hd(XP& p, int rw, int64_t grid, hipStream_t st) {
+  if constexpr (sizeof(T) == 2 && HDP > 64)
+    if (rw == 8) return dkv_shape<T, HDP, 8>(p, grid, st);
+  return rw == 1 ? dkv_shape<T, HDP, 1>(p, grid, st) : rw == 2 ? dkv_shape<T, HDP, 2>(p, grid, st) : dkv_shape<T, HDP, 4>(p, grid, st);
+}
+
+template <typename T>
+int sum_out(const float* part, T* out, int64_t ld, int rows, int width, int nsplit, float f, const int* cu, int batch, hipStream_t st) {
+  int64_t g = cdiv64((int64_t)rows * (width / 4), 256);
+  if (g > 8 * x_cus()) g = 8 * x_cus();
+  hipLaunchKernelGGL((xattn_sum_kernel<T>), dim3((unsigned)g), dim3(256), 0, st, part, out, (long)ld, rows, width, nsplit, f, cu, batch);
+  DH_CHECK_LAUNCH();
   return DH_OK;
 }
 
 #define XATTN_HD(fn, T, ...) \
   (p.hd <= 32 ? fn<T, 32>(__VA_ARGS__) : p.hd <= 64 ? fn<T, 64>(__VA_ARGS__) : p.hd <= 96 ? fn<T, 96>(__VA_ARGS__) : fn<T, 128>(__VA_ARGS__))
 
-int64_t split_bytes(const dh_xattn_args* a, int nsplit) { return nsplit > 1 ? (int64_t)nsplit * a->heads * a->rows_q * (a->hd + 2) * 4 : 0; }
+template <typename T>
+int join_ranges(const XP& p, hipStream_t st) {
+  const int64_t pairs = (int64_t)p.rows_q * p.heads;
+  const bool wide = p.nsplit > 8 && pairs < 4 * x_cus() * 4;
+  int64_t g = wide ? pairs : cdiv64(pairs, 4);
+  if (g > 8 * x_cus()) g = 8 * x_cus();
+  if (wide) hipLaunchKernelGGL((xattn_join_kernel<T, 4>), dim3((unsigned)g), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((xattn_join_kernel<T, 1>), dim3((unsigned)g), dim3(256), 0, st, p);
+  DH_CHECK_LAUNCH();
+  return DH_OK;
+}
+template <typename T>
+int bwd(const dh_xattn_args* a, hipStream_t st) {
+  XP p = params(a);
+  p.delta = (float*)a->ws;
+  p.part_o = p.delta + round4((int64_t)a->heads * a->rows_q);
+  int64_t grid;
+  if (a->rows_q > 0) {
+    const Plan pl = plan_dq(a);
+    if (int e = lay_out(p, pl.tiles, pl.nsplit, a->cu_q != nullptr, grid)) return e;
+    if (int e = XATTN_HD(dq_hd, T, p, pl.rw, grid, st)) return e;
+    if (pl.nsplit > 1)
+      if (int e = sum_out<T>(p.part_o, (T*)a->dq, a->lddq, a->rows_q, a->heads * a->hd, pl.nsplit, a->scale, a->cu_q, a->batch, st)) return e;
+  }
+  if (a->rows_kv > 0) {
+    const Plan pl = plan_dkv(a);
+    if (int e = lay_out(p, pl.tiles, pl.nsplit, a->cu_kv != nullptr, grid)) return e;
+    if (int e = XATTN_HD(dkv_hd, T, p, pl.rw, grid, st)) return e;
+    if (pl.nsplit > 1) {
+      const int width = a->kv_heads * a->hd;
+      if (int e = sum_out<T>(p.part_o, (T*)a->dk, a->lddk, a->rows_kv, width, pl.nsplit, a->scale, a->cu_kv, a->batch, st)) return e;
+      return sum_out<T>(p.part_o + (int64_t)pl.nsplit * a->rows_kv * width, (T*)a->dv, a->lddv, a->rows_kv, width, pl.nsplit, 1.f, a->cu_kv, a->batch, st);
+    }
+  }
+  return DH_OK;
+}
+
+int64_t fwd_bytes(const dh_xattn_args* a) {
+  const int64_t ns = plan_fwd(a).nsplit;
+  return ns > 1 ? ns * a->heads * a->rows_q * (a->hd + 2) * 4 : 0;
+}
+int64_t bwd_bytes(const dh_xattn_args* a) {       // D, and the larger of the partial dq and the partial dk, dv
+  const int64_t sq = plan_dq(a).nsplit, sk = plan_dkv(a).nsplit;
+  const int64_t q = sq > 1 ? sq * a->rows_q * a->heads * a->hd : 0, kv = sk > 1 ? 2 * sk * a->rows_kv * a->kv_heads * a->hd : 0;
+  return (round4((int64_t)a->heads * a->rows_q) + (q > kv ? q : kv)) * 4;
+}
 
 }  // namespace
 
 extern "C" int64_t dh_xattn_ws_bytes(const dh_xattn_args* a, int backward) {
-  if (check_args(a, "dh_xattn_ws_bytes", false) == DH_ERR_ARG && (!a || a->batch <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->heads % a->kv_heads != 0)) return -1;
-  if (backward) return (int64_t)a->heads * a->rows_q * 4;
-  return split_bytes(a, plan_fwd(a).nsplit);
+  if (check_geometry(a, "dh_xattn_ws_bytes")) return -1;
+  return backward ? bwd_bytes(a) : fwd_bytes(a);
 }
 
 extern "C" int dh_xattn_fwd(const dh_xattn_args* a, dh_stream_t stream) {
@@ -850,7 +994,7 @@ extern "C" int dh_xattn_fwd(const dh_xattn_args* a, dh_stream_t stream) {
   if (a->rows_q == 0) return DH_OK;
   const Plan pl = plan_fwd(a);
   XP p = params(a);
-  const int64_t need = split_bytes(a, pl.nsplit);
+  const int64_t need = fwd_bytes(a);
   DH_REQUIRE(need == 0 || (a->ws && a->ws_bytes >= need && ((uintptr_t)a->ws & 15) == 0), "dh_xattn_fwd: workspace of %lld bytes needed", (long long)need);
   if (need) {
     p.part_o = (float*)a->ws;
@@ -858,21 +1002,14 @@ extern "C" int dh_xattn_fwd(const dh_xattn_args* a, dh_stream_t stream) {
   }
   int64_t grid;
   if (int e = lay_out(p, pl.tiles, pl.nsplit, a->cu_q != nullptr, grid)) return e;
-  const int rc = a->dtype == DH_BF16 ? XATTN_HD(fwd_hd, bf16_t, p, pl, grid, (hipStream_t)stream) : XATTN_HD(fwd_hd, float, p, pl, grid, (hipStream_t)stream);
+  const int rc = a->dtype == DH_BF16 ? XATTN_HD(fwd_hd, bf16_t, p, pl.rw, grid, (hipStream_t)stream) : XATTN_HD(fwd_hd, float, p, pl.rw, grid, (hipStream_t)stream);
   if (rc || pl.nsplit == 1) return rc;
-  int64_t jg = cdiv64((int64_t)a->rows_q * a->heads, 4);
-  if (jg > 8 * x_cus()) jg = 8 * x_cus();
-  if (a->dtype == DH_BF16) hipLaunchKernelGGL(xattn_join_kernel<bf16_t>, dim3((unsigned)jg), dim3(256), 0, (hipStream_t)stream, p);
-  else hipLaunchKernelGGL(xattn_join_kernel<float>, dim3((unsigned)jg), dim3(256), 0, (hipStream_t)stream, p);
-  DH_CHECK_LAUNCH();
-  return DH_OK;
+  return a->dtype == DH_BF16 ? join_ranges<bf16_t>(p, (hipStream_t)stream) : join_ranges<float>(p, (hipStream_t)stream);
 }
 
 extern "C" int dh_xattn_bwd(const dh_xattn_args* a, dh_stream_t stream) {
   if (int e = check_args(a, "dh_xattn_bwd", true)) return e;
-  const int64_t need = (int64_t)a->heads * a->rows_q * 4;
+  const int64_t need = bwd_bytes(a);
   DH_REQUIRE(need == 0 || (a->ws && a->ws_bytes >= need && ((uintptr_t)a->ws & 15) == 0), "dh_xattn_bwd: workspace of %lld bytes needed", (long long)need);
-  XP p = params(a);
-  p.delta = (float*)a->ws;
-  return a->dtype == DH_BF16 ? XATTN_HD(bwd_hd, bf16_t, p, a, (hipStream_t)stream) : XATTN_HD(bwd_hd, float, p, a, (hipStream_t)stream);
+  return a->dtype == DH_BF16 ? bwd<bf16_t>(a, (hipStream_t)stream) : bwd<float>(a, (hipStream_t)stream);
 }

@@ -943,8 +943,11 @@ def _xattn_plan(q, k, v, heads, kv_heads, batch, n_q, n_kv, scale, max_q, max_kv
     # the tables' presence decides the workspace, their place does not
     probe = L.XattnArgs.from_buffer_copy(a)
     probe.cu_q, probe.cu_kv = (None if n is None else 16 for n in (n_q, n_kv))
-    need = L.load().dh_xattn_ws_bytes(ctypes.byref(probe), 0)
-    return a, max(int(need), 0)
+    lib = L.load()
+    need = [lib.dh_xattn_ws_bytes(ctypes.byref(probe), backward) for backward in (0, 1)]
+    if min(need) < 0:
+        check(-1, "dh_xattn")
+    return a, need
 
 
 def _xattn_call(q, k, v, heads, kv_heads, batch, cu_q, cu_kv, kv_len, key_mask, scale, max_q, max_kv):
@@ -981,9 +984,9 @@ def xattn_fwd(q, k, v, heads, *, kv_heads=None, batch=None, cu_q=None, cu_kv=Non
     out = torch.empty(a.rows_q, a.ldo, device=on, dtype=q.dtype)
     lse = torch.empty(a.heads, a.rows_q, device=on, dtype=torch.float32)
     a.out, a.lse = out.data_ptr(), lse.data_ptr()
-    if need:
-        ws = torch.empty(need // 4, device=on, dtype=torch.float32)
-        a.ws, a.ws_bytes = ws.data_ptr(), need
+    if need[0]:
+        ws = torch.empty(need[0] // 4, device=on, dtype=torch.float32)
+        a.ws, a.ws_bytes = ws.data_ptr(), need[0]
     check(L.load().dh_xattn_fwd(ctypes.byref(a), _stream_on(dev)), "dh_xattn_fwd")
     return out, lse
 
@@ -995,7 +998,7 @@ def xattn_bwd(q, k, v, out, dout, lse, heads, *, kv_heads=None, batch=None, cu_q
         with torch.cuda.device(dev):
             return xattn_bwd(q, k, v, out, dout, lse, heads, kv_heads=kv_heads, batch=batch, cu_q=cu_q, cu_kv=cu_kv, kv_len=kv_len, key_mask=key_mask, scale=scale,
                              max_q=max_q, max_kv=max_kv)
-    a, _ = _xattn_call(q, k, v, heads, kv_heads, batch, cu_q, cu_kv, kv_len, key_mask, scale, max_q, max_kv)
+    a, need = _xattn_call(q, k, v, heads, kv_heads, batch, cu_q, cu_kv, kv_len, key_mask, scale, max_q, max_kv)
     if not (out.shape == q.shape == dout.shape and out.dtype == q.dtype == dout.dtype):
         raise L.DeclipHipError("bad argument: out and dout like q")
     if lse.shape != (a.heads, a.rows_q) or lse.dtype is not torch.float32 or not lse.is_contiguous():
@@ -1003,11 +1006,11 @@ def xattn_bwd(q, k, v, out, dout, lse, heads, *, kv_heads=None, batch=None, cu_q
     on = q.device
     dq = torch.empty(a.rows_q, a.lddq, device=on, dtype=q.dtype)
     dk, dv = (torch.empty(a.rows_kv, a.lddk, device=on, dtype=q.dtype) for _ in range(2))
-    ws = torch.empty(max(a.heads * a.rows_q, 4), device=on, dtype=torch.float32)      # = dh_xattn_ws_bytes(args, 1)
+    ws = torch.empty(max(need[1], 16) // 4, device=on, dtype=torch.float32)
     a.out, a.ldo, a.lse = out.data_ptr(), _row_stride(out, "out"), lse.data_ptr()
     a.dout, a.lddo = dout.data_ptr(), _row_stride(dout, "dout")
     a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-    a.ws, a.ws_bytes = ws.data_ptr(), ws.numel() * 4
+    a.ws, a.ws_bytes = ws.data_ptr(), need[1]
     check(L.load().dh_xattn_bwd(ctypes.byref(a), _stream_on(dev)), "dh_xattn_bwd")
     return dq, dk, dv
 
