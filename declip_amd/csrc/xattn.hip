@@ -42,6 +42,14 @@ struct XP {
   int by_pair;        // block order: 1 = the blocks of one (sequence, kv head) on one XCD
 };
 
+// Tiles in LDS: row-major, rows padded so that 16 consecutive rows at one 16-byte chunk (the row operand) start in 16 different groups of 4 banks and 4
+// consecutive rows (the transpose read, 64 bytes of each) overlap as little as such a stride allows.  (Conflict-free for both would be an exclusive-or of the
+// chunk with the row; its address registers spill: hd 128 dq 191 -> 213 us, dkv 382 -> 453.  128 columns padded by 8 instead of 24: fwd 159 us against 150,
+// dkv 384 against 350.)
+template <typename T, int HDP> struct Lay {
+  static constexpr int EPC = 16 / sizeof(T), LD = HDP + (sizeof(T) == 2 && HDP == 128 ? 24 : EPC);
+};
+
 template <typename T> struct Op;
 template <> struct Op<bf16_t> {
   static constexpr int EPC = 8;                      // elements of a 16-byte chunk
@@ -60,8 +68,10 @@ template <> struct Op<bf16_t> {
     return p;
   }
   // c[32 columns col0.. of the tile] += tile rows row0 .. row0 + 31, transposed, times p
-  static __device__ __forceinline__ void mma_t(f32x16_t& c, const bf16_t* tile, int ld, int row0, int col0, const PF& p, int lane) {
+  template <int HDP>
+  static __device__ __forceinline__ void mma_t(f32x16_t& c, const bf16_t* tile, int row0, int col0, const PF& p, int lane) {
     typedef __attribute__((ext_vector_type(4))) short s16x4;
+    constexpr int ld = Lay<bf16_t, HDP>::LD;
     const int t16 = lane & 15;
     const bf16_t* b = tile + (row0 + 4 * (lane >> 5) + (t16 >> 2)) * ld + col0 + 16 * ((lane >> 4) & 1) + 4 * (t16 & 3);
 #pragma unroll
@@ -98,7 +108,9 @@ template <> struct Op<float> {
     for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
   }
   static __device__ __forceinline__ PF pack(const f32x16_t& s) { return s; }
-  static __device__ __forceinline__ void mma_t(f32x16_t& c, const float* tile, int ld, int row0, int col0, const PF& p, int lane) {
+  template <int HDP>
+  static __device__ __forceinline__ void mma_t(f32x16_t& c, const float* tile, int row0, int col0, const PF& p, int lane) {
+    constexpr int ld = Lay<float, HDP>::LD;
     const float* b = tile + (row0 + 4 * (lane >> 5)) * ld + col0 + (lane & 31);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -204,12 +216,12 @@ __device__ __forceinline__ void load_row(typename Op<T>::Frag* f, const T* row, 
   }
 }
 template <typename T, int HDP>
-__device__ __forceinline__ f32x16_t mma_row(const T* tile, int ld, int row0, const typename Op<T>::Frag* f, int lane) {
+__device__ __forceinline__ f32x16_t mma_row(const T* tile, int row0, const typename Op<T>::Frag* f, int lane) {
   constexpr int EPC = Op<T>::EPC, KS = HDP / (2 * EPC);
   f32x16_t c;
 #pragma unroll
   for (int i = 0; i < 16; ++i) c[i] = 0.f;
-  const T* row = tile + (row0 + (lane & 31)) * ld + (lane >> 5) * EPC;
+  const T* row = tile + (row0 + (lane & 31)) * Lay<T, HDP>::LD + (lane >> 5) * EPC;
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) Op<T>::mma(c, *reinterpret_cast<const typename Op<T>::Frag*>(row + ks * 2 * EPC), f[ks]);
   return c;
@@ -237,7 +249,7 @@ __device__ __forceinline__ float half_max(float v) {
 // branch: rows behind the last one read that one again), store() puts it into the other LDS buffer one iteration later.
 template <typename T, int HDP, int ROWS, int NT>
 struct Pair2 {
-  static constexpr int EPC = Op<T>::EPC, NCH = HDP / EPC, N = (ROWS * NCH + NT - 1) / NT, LD = HDP + EPC;
+  static constexpr int EPC = Op<T>::EPC, NCH = HDP / EPC, N = (ROWS * NCH + NT - 1) / NT, LD = Lay<T, HDP>::LD;
   static constexpr bool RAGGED = ROWS * NCH % NT != 0;      // fewer tasks than threads, or a last round of fewer
   uint4 a[N], b[N];
   uint8_t keep[N];
@@ -270,7 +282,7 @@ struct Pair2 {
 // The key tiles of a sequence: K and V rows in two LDS buffers, the validity of their keys beside them.
 template <typename T, int HDP, int BN, int NT>
 struct Tiles {
-  static constexpr int LD = HDP + Op<T>::EPC;
+  static constexpr int LD = Lay<T, HDP>::LD;
   const T *kb, *vb;
   const uint8_t* km;
   T* buf;
@@ -356,9 +368,9 @@ __device__ __forceinline__ void rows_out(unsigned char* smem, const f32x16_t* ac
 // rescaled forward 192 instructions a tile) unless that spills more than it hides.  Measured in us, 256 captions of 5 .. 77 tokens on 197 keys, 8 heads:
 // hd 128 dq 1 wave per block 87 for one wave per SIMD against 262 for two, dkv of 2 waves per block 180 / 370, of 4 waves 194 / 276; hd 96 (128 sequences
 // of 77) dkv of 4 waves 97 / 79; fp32 hd 64 (16 sequences of 77) dkv 23 / 29, fwd of one wave 17.6 / 23.  RW: waves per block.
-template <typename T, int HDP, int RW> constexpr int waves_fwd() {
+template <typename T, int HDP, int RW, bool SPLIT> constexpr int waves_fwd() {
   constexpr int row = HDP * sizeof(T);
-  return RW == 1 ? (row <= 64 ? 3 : sizeof(T) == 2 && row <= 128 ? 2 : 1) : RW == 2 ? (row <= 128 ? 3 : row <= 256 ? 2 : 1) : row <= 384 ? 2 : 1;
+  return SPLIT && RW == 4 && row <= 128 && sizeof(T) == 2 ? 3 : RW == 1 ? (row <= 64 ? 3 : sizeof(T) == 2 && row <= 128 ? 2 : 1) : RW == 2 ? (row <= 128 ? 3 : row <= 256 ? 2 : 1) : row <= 384 ? 2 : 1;
 }
 template <typename T, int HDP, int RW> constexpr int waves_dq() {
   constexpr int row = HDP * sizeof(T);
@@ -371,8 +383,8 @@ template <typename T, int HDP, int RW> constexpr int waves_dkv() {
 
 // ------------------------------------------------------------------------------------------ forward
 template <typename T, int HDP, int RW, int BN, bool SPLIT>
-__global__ __launch_bounds__(64 * RW, (waves_fwd<T, HDP, RW>())) void xattn_fwd_kernel(XP p) {
-  constexpr int EPC = Op<T>::EPC, LD = HDP + EPC, KS = HDP / (2 * EPC), DB = HDP / 32, NB = BN / 32, BM = 32 * RW, NT = 64 * RW;
+__global__ __launch_bounds__(64 * RW, (waves_fwd<T, HDP, RW, SPLIT>())) void xattn_fwd_kernel(XP p) {
+  constexpr int EPC = Op<T>::EPC, KS = HDP / (2 * EPC), DB = HDP / 32, NB = BN / 32, BM = 32 * RW, NT = 64 * RW;
   DH_DYN_LDS_A16(unsigned char, smem);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
   if ((int)blockIdx.x >= p.main_blocks) {
@@ -419,8 +431,10 @@ __global__ __launch_bounds__(64 * RW, (waves_fwd<T, HDP, RW>())) void xattn_fwd_
       const bool masked = kt_.next(kt, hi, tid, Ks, Vs, bias);
       if (wave_live) {
         f32x16_t sc[NB];
+        __builtin_amdgcn_s_setprio(1);                 // (the wave at its products goes before the one at its softmax: 162 -> 158 us for 16 pairs of 4096 on 3136, hd 128)
 #pragma unroll
-        for (int b = 0; b < NB; ++b) sc[b] = mma_row<T, HDP>(Ks, LD, b * 32, qf, lane);
+        for (int b = 0; b < NB; ++b) sc[b] = mma_row<T, HDP>(Ks, b * 32, qf, lane);
+        __builtin_amdgcn_s_setprio(0);
         if (masked) {
 #pragma unroll
           for (int b = 0; b < NB; ++b) mask_keys(sc[b], bias + b * 32, h);
@@ -453,12 +467,14 @@ __global__ __launch_bounds__(64 * RW, (waves_fwd<T, HDP, RW>())) void xattn_fwd_
             sum += e;
           }
         l += sum;                                      // this half-wave's keys; joined behind the loop
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
           const typename Op<T>::PF pf = Op<T>::pack(sc[b]);
 #pragma unroll
-          for (int d = 0; d < DB; ++d) Op<T>::mma_t(o[d], Vs, LD, b * 32, d * 32, pf, lane);
+          for (int d = 0; d < DB; ++d) Op<T>::template mma_t<HDP>(o[d], Vs, b * 32, d * 32, pf, lane);
         }
+        __builtin_amdgcn_s_setprio(0);
       }
       __syncthreads();                                 // this buffer is read, the other one written
     }
@@ -477,18 +493,46 @@ __global__ __launch_bounds__(64 * RW, (waves_fwd<T, HDP, RW>())) void xattn_fwd_
   }
 }
 
-// joins the key ranges of one (query row, head): o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, in a fixed order.  JW waves per pair (4: many ranges, few
-// pairs) take every JW-th range; their lanes read the ranges' (m, l) at once, and a lane's columns of eight partial sums are independent loads.
-template <typename T, int JW>
+// Joins the key ranges of a (query row, head): o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, in a fixed order.
+// Few ranges: a thread per 4 columns, all of its loads independent.
+template <typename T>
 __global__ __launch_bounds__(256) void xattn_join_kernel(XP p) {
+  int first = 0, last = p.rows_q;
+  if (p.cu_q) owned(p.cu_q, p.batch, p.rows_q, first, last);
+  const int nch = p.hd / 4;
+  const long n = (long)(last - first) * p.heads * nch, stride = (long)p.heads * p.rows_q;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
+    const long pair = i / nch;
+    const int c = (int)(i - pair * nch) * 4, row = first + (int)(pair / p.heads), head = (int)(pair % p.heads);
+    const long stat = (long)head * p.rows_q + row;
+    float m = -INFINITY;
+#pragma unroll 4
+    for (int s = 0; s < p.nsplit; ++s) m = fmaxf(m, p.part_ml[2 * (s * stride + stat)]);
+    const float ms = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = 0; s < p.nsplit; ++s) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * (s * stride + stat));
+      const float4 v = *reinterpret_cast<const float4*>(p.part_o + (s * stride + stat) * p.hd + c);
+      const float f = exp2_fast(ml.x - ms);
+      l = fmaf(f, ml.y, l);
+      if (ml.y != 0.f) { o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w); }   // (an empty range wrote no sums)
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    Op<T>::store4((T*)p.out + (long)row * p.ldo + (long)head * p.hd + c, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    if (c == 0) p.lse[stat] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
+  }
+}
+// Many ranges of few pairs: a block per pair, its waves take every fourth range, eight loads of a lane at a time.
+template <typename T>
+__global__ __launch_bounds__(256) void xattn_join_many_kernel(XP p) {
   __shared__ float2 part_sum[4][64];
   int first = 0, last = p.rows_q;
   if (p.cu_q) owned(p.cu_q, p.batch, p.rows_q, first, last);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c0 = 2 * lane, w = JW == 1 ? 0 : wave;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c0 = 2 * lane;
   const long n = (long)(last - first) * p.heads, stride = (long)p.heads * p.rows_q;
-  for (long i0 = (long)blockIdx.x * (4 / JW); i0 < n; i0 += (long)gridDim.x * (4 / JW)) {
-    const long i = i0 + (JW == 1 ? wave : 0);
-    if (JW == 1 && i >= n) break;
+  for (long i = blockIdx.x; i < n; i += gridDim.x) {
     const int row = first + (int)(i / p.heads), head = (int)(i % p.heads);
     const long stat = (long)head * p.rows_q + row;
     float2 ml = make_float2(-INFINITY, 0.f);
@@ -496,31 +540,29 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XP p) {
     const float m = wave_max(ml.x), f = ml.y == 0.f ? 0.f : exp2_fast(ml.x - m), l = wave_sum(f * ml.y);
     float2 acc = make_float2(0.f, 0.f);
     const float* part = p.part_o + stat * p.hd + (c0 < p.hd ? c0 : 0);
-    for (int s0 = w; s0 < p.nsplit; s0 += 8 * JW) {
+    for (int s0 = wave; s0 < p.nsplit; s0 += 32) {
       float2 v[8];
       float fs[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const int s = min(s0 + k * JW, p.nsplit - 1);
+        const int s = min(s0 + 4 * k, p.nsplit - 1);
         v[k] = *reinterpret_cast<const float2*>(part + s * stride * p.hd);
-        fs[k] = s0 + k * JW < p.nsplit ? __shfl(f, s, 64) : 0.f;
+        fs[k] = s0 + 4 * k < p.nsplit ? __shfl(f, s, 64) : 0.f;
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (fs[k] != 0.f) {                          // (an empty range wrote no sums)
+        if (fs[k] != 0.f) {
           acc.x = fmaf(fs[k], v[k].x, acc.x);
           acc.y = fmaf(fs[k], v[k].y, acc.y);
         }
     }
-    if (JW > 1) {
-      __syncthreads();
-      part_sum[wave][lane] = acc;
-      __syncthreads();
-      if (wave) continue;
-      acc = part_sum[0][lane];
+    __syncthreads();
+    part_sum[wave][lane] = acc;
+    __syncthreads();
+    if (wave) continue;
+    acc = part_sum[0][lane];
 #pragma unroll
-      for (int k = 1; k < JW; ++k) { acc.x += part_sum[k][lane].x; acc.y += part_sum[k][lane].y; }
-    }
+    for (int k = 1; k < 4; ++k) { acc.x += part_sum[k][lane].x; acc.y += part_sum[k][lane].y; }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     T* o = (T*)p.out + (long)row * p.ldo + (long)head * p.hd + c0;
     if (c0 < p.hd) { st<T>(o, acc.x * inv); st<T>(o + 1, acc.y * inv); }
@@ -552,7 +594,7 @@ __global__ __launch_bounds__(256) void xattn_sum_kernel(const float* part, T* ou
 // ------------------------------------------------------------------------------------------ backward: dq (and D)
 template <typename T, int HDP, int RW, int BN, bool SPLIT>
 __global__ __launch_bounds__(64 * RW, (waves_dq<T, HDP, RW>())) void xattn_dq_kernel(XP p) {
-  constexpr int EPC = Op<T>::EPC, LD = HDP + EPC, KS = HDP / (2 * EPC), DB = HDP / 32, NB = BN / 32, BM = 32 * RW, NT = 64 * RW;
+  constexpr int EPC = Op<T>::EPC, KS = HDP / (2 * EPC), DB = HDP / 32, NB = BN / 32, BM = 32 * RW, NT = 64 * RW;
   DH_DYN_LDS_A16(unsigned char, smem);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
   if ((int)blockIdx.x >= p.main_blocks) {
@@ -599,8 +641,8 @@ __global__ __launch_bounds__(64 * RW, (waves_dq<T, HDP, RW>())) void xattn_dq_ke
       const bool masked = kt_.next(kt, hi, tid, Ks, Vs, bias);
       const bool busy = wave_live;
       auto p_dp = [&](int b, f32x16_t& sc, f32x16_t& dp) {     // p and dp of 32 keys
-        sc = mma_row<T, HDP>(Ks, LD, b * 32, qf, lane);
-        dp = mma_row<T, HDP>(Vs, LD, b * 32, df, lane);
+        sc = mma_row<T, HDP>(Ks, b * 32, qf, lane);
+        dp = mma_row<T, HDP>(Vs, b * 32, df, lane);
         if (masked) mask_keys(sc, bias + b * 32, h);
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[i] = exp2_fast(fmaf(sc[i], c, -lse2));
@@ -630,7 +672,7 @@ __global__ __launch_bounds__(64 * RW, (waves_dq<T, HDP, RW>())) void xattn_dq_ke
           for (int i = 0; i < 16; ++i) sc[i] *= dp[i] - D;
           const typename Op<T>::PF pf = Op<T>::pack(sc);
 #pragma unroll
-          for (int d = 0; d < DB; ++d) Op<T>::mma_t(dq[d], Ks, LD, b * 32, d * 32, pf, lane);
+          for (int d = 0; d < DB; ++d) Op<T>::template mma_t<HDP>(dq[d], Ks, b * 32, d * 32, pf, lane);
         }
       }
       __syncthreads();
@@ -647,7 +689,7 @@ __global__ __launch_bounds__(64 * RW, (waves_dq<T, HDP, RW>())) void xattn_dq_ke
 // ------------------------------------------------------------------------------------------ backward: dk, dv
 template <typename T, int HDP, int RW, bool SPLIT>
 __global__ __launch_bounds__(64 * RW, (waves_dkv<T, HDP, RW>())) void xattn_dkv_kernel(XP p) {
-  constexpr int EPC = Op<T>::EPC, LD = HDP + EPC, KS = HDP / (2 * EPC), DB = HDP / 32, BQ = 32, BK = 32 * RW, NT = 64 * RW;
+  constexpr int EPC = Op<T>::EPC, LD = Lay<T, HDP>::LD, KS = HDP / (2 * EPC), DB = HDP / 32, BQ = 32, BK = 32 * RW, NT = 64 * RW;
   DH_DYN_LDS_A16(unsigned char, smem);
   T* buf = reinterpret_cast<T*>(smem);                 // two buffers of Q and dO rows, lse and D of the rows
   float* stats = reinterpret_cast<float*>(buf + 4 * BQ * LD);
@@ -717,8 +759,8 @@ __global__ __launch_bounds__(64 * RW, (waves_dkv<T, HDP, RW>())) void xattn_dkv_
       if (wave_live) {
         const T *Qs = buf + (mt & 1) * 2 * BQ * LD, *Ds = Qs + BQ * LD;
         const float *lse2s = stats + (mt & 1) * 2 * BQ, *dels = lse2s + BQ;
-        f32x16_t sc = mma_row<T, HDP>(Qs, LD, 0, kf, lane);
-        f32x16_t dp = mma_row<T, HDP>(Ds, LD, 0, vf, lane);
+        f32x16_t sc = mma_row<T, HDP>(Qs, 0, kf, lane);
+        f32x16_t dp = mma_row<T, HDP>(Ds, 0, vf, lane);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float4 L = *reinterpret_cast<const float4*>(lse2s + 8 * i + 4 * h);
@@ -731,8 +773,8 @@ __global__ __launch_bounds__(64 * RW, (waves_dkv<T, HDP, RW>())) void xattn_dkv_
         const typename Op<T>::PF pf = Op<T>::pack(sc), sf = Op<T>::pack(dp);
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
-          Op<T>::mma_t(dv[d], Ds, LD, 0, d * 32, pf, lane);
-          Op<T>::mma_t(dk[d], Qs, LD, 0, d * 32, sf, lane);
+          Op<T>::template mma_t<HDP>(dv[d], Ds, 0, d * 32, pf, lane);
+          Op<T>::template mma_t<HDP>(dk[d], Qs, 0, d * 32, sf, lane);
         }
       }
       __syncthreads();
@@ -800,7 +842,11 @@ Plan plan_of(const dh_xattn_args* a, Kind kind, int64_t rows, int64_t other, int
   Plan r;
   r.rw = row_waves(a, kind, rows, other);
   r.tiles = (int)cdiv64(rows < 1 ? 1 : rows, 32 * r.rw);
-  const int64_t blocks = (int64_t)r.tiles * a->batch * a->kv_heads, want = (int64_t)x_cus() * (8 / r.rw);
+  // Two waves per SIMD; the forward of up to 64 columns fits three, and with ranges of 1024 keys and more their partial results cost less than they
+  // bring (24 pairs of 2047 on 6272: 161 us whole, 111 + 10 us in two ranges).
+  const bool three = kind == FWD && a->dtype == DH_BF16 && a->hd <= 64 && r.rw == 4 && other >= 2048;
+  const int64_t blocks = (int64_t)r.tiles * a->batch * a->kv_heads, want = (int64_t)x_cus() * ((three ? 12 : 8) / r.rw);
+  if (three) step = 1024;
   int64_t ns = blocks >= want ? 1 : want / blocks;
   const int64_t most = cdiv64(other, step);
   if (ns > most) ns = most;
@@ -881,7 +927,7 @@ int launch(K kernel, const XP& p, int64_t grid, int threads, size_t lds, hipStre
 
 // LDS of a block: two buffers of two tiles with `per_row` floats beside each tile row; the result rows go through it at the end (fp32 where split)
 template <typename T, int HDP, int RW> constexpr size_t lds_bytes(int rows, int per_row, bool split) {
-  const size_t tiles = 2 * ((size_t)2 * rows * (HDP + Op<T>::EPC) * sizeof(T) + (size_t)rows * per_row * 4);
+  const size_t tiles = 2 * ((size_t)2 * rows * Lay<T, HDP>::LD * sizeof(T) + (size_t)rows * per_row * 4);
   const size_t out = split || sizeof(T) == 4 ? (size_t)RW * 32 * (HDP + 4) * 4 : (size_t)RW * 32 * (HDP + Op<T>::EPC) * sizeof(T);
   return tiles > out ? tiles : out;
 }
@@ -938,11 +984,13 @@ int sum_out(const float* part, T* out, int64_t ld, int rows, int width, int nspl
 template <typename T>
 int join_ranges(const XP& p, hipStream_t st) {
   const int64_t pairs = (int64_t)p.rows_q * p.heads;
-  const bool wide = p.nsplit > 8 && pairs < 4 * x_cus() * 4;
-  int64_t g = wide ? pairs : cdiv64(pairs, 4);
-  if (g > 8 * x_cus()) g = 8 * x_cus();
-  if (wide) hipLaunchKernelGGL((xattn_join_kernel<T, 4>), dim3((unsigned)g), dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((xattn_join_kernel<T, 1>), dim3((unsigned)g), dim3(256), 0, st, p);
+  if (p.nsplit > 8 && pairs < 16 * x_cus()) {
+    hipLaunchKernelGGL((xattn_join_many_kernel<T>), dim3((unsigned)(pairs < 8 * x_cus() ? pairs : 8 * x_cus())), dim3(256), 0, st, p);
+  } else {
+    int64_t g = cdiv64(pairs * (p.hd / 4), 256);
+    if (g > 32 * x_cus()) g = 32 * x_cus();
+    hipLaunchKernelGGL((xattn_join_kernel<T>), dim3((unsigned)g), dim3(256), 0, st, p);
+  }
   DH_CHECK_LAUNCH();
   return DH_OK;
 }
