@@ -330,7 +330,7 @@ __global__ __launch_bounds__(NT, 2) void join_bwd_kernel(JP p) {
   for (int row0 = first; row0 < last; row0 += G) {
     const int row = row0 + ln.group;
     const bool live = row < last;
-    const float rs = nst[1], mr = -nst[0] * nst[1], rs2 = nst[3], mr2 = -nst[2] * nst[3], g = ROWGATE ? act(p, ng) : 1.f;
+    const float mu = nst[0], rs = nst[1], mu2 = nst[2], rs2 = nst[3], g = ROWGATE ? act(p, ng) : 1.f;
     float yh[NC][V], Gr[NC][V], xh[NC][V], wn[NC][V];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
@@ -343,9 +343,9 @@ __global__ __launch_bounds__(NT, 2) void join_bwd_kernel(JP p) {
       nn[k].get(dnv);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        yh[k][e] = fmaf(yh[k][e], rs, mr);
+        yh[k][e] = (yh[k][e] - mu) * rs;
         const float t = fmaf(yh[k][e], sw[e], sb[e]);
-        xh[k][e] = fmaf(fmaf(p.alpha, xv[e], ROWGATE ? g * t : t), rs2, mr2);
+        xh[k][e] = (fmaf(p.alpha, xv[e], ROWGATE ? g * t : t) - mu2) * rs2;
         wn[k][e] = dnv[e] * pw[e];              // (0 behind column d and without dn)
         s1 += wn[k][e];
         s2 = fmaf(wn[k][e], xh[k][e], s2);
@@ -549,10 +549,11 @@ int bwd_blocks(const dh_join_norm_args* a, int w, int& per_group) { return block
 int check(const dh_join_norm_args* a, const char* who) {
   DH_REQUIRE(a, "%s: null args", who);
   DH_REQUIRE(a->dtype == DH_F32 || a->dtype == DH_BF16, "%s: dtype %d", who, a->dtype);
-  DH_REQUIRE(a->rows >= 0 && a->d > 0 && a->d <= 8192, "%s: rows %d, width %d (up to 8192)", who, a->rows, a->d);
+  DH_REQUIRE(a->rows >= 0 && a->rows < (1 << 30) && a->d > 0 && a->d <= 8192, "%s: rows %d (below 2^30), width %d (up to 8192)", who, a->rows, a->d);
   DH_REQUIRE(!a->post_b || (a->post_w && !a->rms), "%s: a bias needs its weight and a LayerNorm", who);
   DH_REQUIRE(!a->pre_b || (a->pre_w && !a->rms), "%s: a bias needs its weight and a LayerNorm", who);
   DH_REQUIRE(!a->gate || (a->gate_rows > 0 && a->rows % a->gate_rows == 0), "%s: %d gate rows for %d rows", who, a->gate_rows, a->rows);
+  DH_REQUIRE(!a->gate || !a->gate_channel || a->gate_rows < (1 << 22), "%s: %d gate vectors (below 2^22)", who, a->gate_rows);
   DH_REQUIRE(a->eps >= 0.f && a->eps < INFINITY, "%s: eps", who);
   DH_REQUIRE(a->rows == 0 || (a->x && a->y && a->stats), "%s: x, y and stats are needed", who);
   return DH_OK;

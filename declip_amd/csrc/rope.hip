@@ -150,9 +150,9 @@ extern "C" int dh_rope_axes(const dh_rope_plan* plan, int dtype, const void* x, 
                             int pos_float, int pos_rows, int inverse, dh_stream_t stream) {
   DH_REQUIRE(plan && plan->axes > 0 && plan->axes <= 8 && plan->pairs > 0 && plan->pairs <= MAX_PAIRS && plan->hd >= 2 * plan->pairs, "dh_rope_axes: plan not initialised");
   DH_REQUIRE(dtype == DH_F32 || dtype == DH_BF16, "dh_rope_axes: dtype %d", dtype);
-  DH_REQUIRE(rows >= 0 && heads > 0, "dh_rope_axes: rows %d, heads %d", rows, heads);
+  DH_REQUIRE(rows >= 0 && rows < (1 << 30) && heads > 0, "dh_rope_axes: rows %d (below 2^30), heads %d", rows, heads);
   const int64_t width = (int64_t)heads * plan->hd;
-  DH_REQUIRE(width < (1 << 30) && (rows <= 1 || (ldx >= width && ldy >= width)), "dh_rope_axes: row strides %lld, %lld for %d heads of %d", (long long)ldx, (long long)ldy, heads, plan->hd);
+  DH_REQUIRE(width < (1 << 27) && (rows <= 1 || (ldx >= width && ldy >= width)), "dh_rope_axes: row strides %lld, %lld for %d heads of %d", (long long)ldx, (long long)ldy, heads, plan->hd);
   if (rows == 0) return DH_OK;
   DH_REQUIRE(x && y && pos && pos_rows > 0 && rows % pos_rows == 0, "dh_rope_axes: %d rows, %d positions", rows, pos_rows);
   RopeP p;

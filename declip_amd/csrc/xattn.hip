@@ -905,13 +905,14 @@ XP params(const dh_xattn_args* a) {
 }
 
 // grid of a kernel over (sequence, kv head) pairs; `clear`: blocks behind it for the rows no sequence owns
-int lay_out(XP& p, int tiles, int nsplit, bool clear, int64_t& grid) {
+int lay_out(XP& p, const Plan& pl, bool clear, int64_t& grid) {
+  const int tiles = pl.tiles, nsplit = pl.nsplit;
   const int64_t pairs = (int64_t)p.batch * p.kv_heads;
   p.tiles = tiles < 1 ? 1 : tiles;
   p.nsplit = nsplit;
   p.by_pair = pairs % 8 == 0 || pairs >= 64;
   const int64_t main = (p.by_pair ? cdiv64(pairs, 8) * 8 : pairs) * p.tiles * nsplit;
-  DH_REQUIRE(main < (1ll << 30), "dh_xattn: grid of %lld blocks", (long long)main);
+  DH_REQUIRE((main + 64) * 64 * pl.rw < (1ll << 32), "dh_xattn: grid of %lld blocks", (long long)main);      // (a launch holds 2^32 threads)
   p.main_blocks = (int)main;
   grid = main + (clear ? 64 : 0);
   return DH_OK;
@@ -1002,14 +1003,14 @@ int bwd(const dh_xattn_args* a, hipStream_t st) {
   int64_t grid;
   if (a->rows_q > 0) {
     const Plan pl = plan_dq(a);
-    if (int e = lay_out(p, pl.tiles, pl.nsplit, a->cu_q != nullptr, grid)) return e;
+    if (int e = lay_out(p, pl, a->cu_q != nullptr, grid)) return e;
     if (int e = XATTN_HD(dq_hd, T, p, pl.rw, grid, st)) return e;
     if (pl.nsplit > 1)
       if (int e = sum_out<T>(p.part_o, (T*)a->dq, a->lddq, a->rows_q, a->heads * a->hd, pl.nsplit, a->scale, a->cu_q, a->batch, st)) return e;
   }
   if (a->rows_kv > 0) {
     const Plan pl = plan_dkv(a);
-    if (int e = lay_out(p, pl.tiles, pl.nsplit, a->cu_kv != nullptr, grid)) return e;
+    if (int e = lay_out(p, pl, a->cu_kv != nullptr, grid)) return e;
     if (int e = XATTN_HD(dkv_hd, T, p, pl.rw, grid, st)) return e;
     if (pl.nsplit > 1) {
       const int width = a->kv_heads * a->hd;
@@ -1049,7 +1050,7 @@ extern "C" int dh_xattn_fwd(const dh_xattn_args* a, dh_stream_t stream) {
     p.part_ml = p.part_o + (int64_t)pl.nsplit * a->heads * a->rows_q * a->hd;
   }
   int64_t grid;
-  if (int e = lay_out(p, pl.tiles, pl.nsplit, a->cu_q != nullptr, grid)) return e;
+  if (int e = lay_out(p, pl, a->cu_q != nullptr, grid)) return e;
   const int rc = a->dtype == DH_BF16 ? XATTN_HD(fwd_hd, bf16_t, p, pl.rw, grid, (hipStream_t)stream) : XATTN_HD(fwd_hd, float, p, pl.rw, grid, (hipStream_t)stream);
   if (rc || pl.nsplit == 1) return rc;
   return a->dtype == DH_BF16 ? join_ranges<bf16_t>(p, (hipStream_t)stream) : join_ranges<float>(p, (hipStream_t)stream);

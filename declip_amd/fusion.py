@@ -17,11 +17,11 @@ from . import ops
 
 
 def _rows16(t):
-    """contiguous columns, 16-byte aligned rows: what the kernels read; anything else is copied"""
+    """contiguous columns, 16-byte aligned rows less than 2^22 elements apart: what the kernels read; anything else is copied"""
     unit = 16 // t.element_size()
     ok = t.dim() == 2 and (t.shape[1] == 1 or t.stride(1) == 1) and t.data_ptr() % 16 == 0
     if ok and t.shape[0] > 1:
-        ok = t.stride(0) >= t.shape[1] and t.stride(0) % unit == 0
+        ok = t.shape[1] <= t.stride(0) < 1 << 22 and t.stride(0) % unit == 0
     return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 

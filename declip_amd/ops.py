@@ -886,6 +886,11 @@ def _plan(key, make):
     return plan
 
 
+def _plain(kind, v):
+    """a plain number, also of a tensor of one element: a plan is found by values, never by what a tensor held when it was made"""
+    return None if v is None else kind(v)
+
+
 def _device_of(t, *others):
     """the device index of a call's tensors (-1: not on a HIP device, which ptr() refuses); all of them lie on one device"""
     dev = t.get_device()
@@ -922,8 +927,7 @@ def _i32_table(t, name, n):
 
 
 def _xattn_plan(q, k, v, heads, kv_heads, batch, n_q, n_kv, scale, max_q, max_kv):
-    heads = int(heads)
-    kv_heads = heads if kv_heads is None else int(kv_heads)
+    kv_heads = heads if kv_heads is None else kv_heads
     _req(q.dim() == 2 and heads > 0 and kv_heads > 0 and heads % kv_heads == 0 and q.shape[1] % heads == 0, "q [rows, heads * hd], heads a multiple of kv_heads")
     hd = q.shape[1] // heads
     for n in (n_q, n_kv):
@@ -934,9 +938,11 @@ def _xattn_plan(q, k, v, heads, kv_heads, batch, n_q, n_kv, scale, max_q, max_kv
     _req(q.dtype == k.dtype == v.dtype, "q, k, v of one dtype")
     _req(k.shape == v.shape, "k and v of one shape")
     a = L.XattnArgs()
-    a.dtype, a.batch, a.heads, a.kv_heads, a.hd = dt(q), int(batch), heads, kv_heads, hd
-    a.rows_q, a.rows_kv, a.max_q, a.max_kv = q.shape[0], k.shape[0], int(max_q or 0), int(max_kv or 0)
-    a.scale = float(scale) if scale is not None else hd ** -0.5
+    for n in (batch, q.shape[0], k.shape[0], q.shape[1], k.shape[1]):
+        _req(n < 1 << 30, "q, k, v: sizes below 2^30")
+    a.dtype, a.batch, a.heads, a.kv_heads, a.hd = dt(q), batch, heads, kv_heads, hd
+    a.rows_q, a.rows_kv, a.max_q, a.max_kv = q.shape[0], k.shape[0], min(max_q or 0, q.shape[0]), min(max_kv or 0, k.shape[0])
+    a.scale = scale if scale is not None else hd ** -0.5
     a.ldq, a.ldk, a.ldv = _row_stride(q, "q"), _row_stride(k, "k", kv_heads * hd), _row_stride(v, "v", kv_heads * hd)
     a.ldo = a.lddo = a.lddq = q.shape[1]
     a.lddk = a.lddv = k.shape[1]
@@ -950,9 +956,11 @@ def _xattn_plan(q, k, v, heads, kv_heads, batch, n_q, n_kv, scale, max_q, max_kv
     return a, need
 
 
-def _xattn_call(q, k, v, heads, kv_heads, batch, cu_q, cu_kv, kv_len, key_mask, scale, max_q, max_kv):
+def _xattn_call(dev, q, k, v, heads, kv_heads, batch, cu_q, cu_kv, kv_len, key_mask, scale, max_q, max_kv):
     n_q, n_kv = None if cu_q is None else cu_q.numel(), None if cu_kv is None else cu_kv.numel()
-    key = ("xattn", q.dtype, k.dtype, v.dtype, q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), heads, kv_heads, batch, n_q, n_kv, scale, max_q, max_kv)
+    if not (scale is None or type(scale) is float) or not all(n is None or type(n) is int for n in (heads, kv_heads, batch, max_q, max_kv)):
+        scale, (heads, kv_heads, batch, max_q, max_kv) = _plain(float, scale), (_plain(int, n) for n in (heads, kv_heads, batch, max_q, max_kv))
+    key = ("xattn", dev, q.dtype, k.dtype, v.dtype, q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), heads, kv_heads, batch, n_q, n_kv, scale, max_q, max_kv)
     plan, need = _plan(key, lambda: _xattn_plan(q, k, v, heads, kv_heads, batch, n_q, n_kv, scale, max_q, max_kv))
     a = L.XattnArgs.from_buffer_copy(plan)
     a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
@@ -979,7 +987,7 @@ def xattn_fwd(q, k, v, heads, *, kv_heads=None, batch=None, cu_q=None, cu_kv=Non
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return xattn_fwd(q, k, v, heads, kv_heads=kv_heads, batch=batch, cu_q=cu_q, cu_kv=cu_kv, kv_len=kv_len, key_mask=key_mask, scale=scale, max_q=max_q, max_kv=max_kv)
-    a, need = _xattn_call(q, k, v, heads, kv_heads, batch, cu_q, cu_kv, kv_len, key_mask, scale, max_q, max_kv)
+    a, need = _xattn_call(dev, q, k, v, heads, kv_heads, batch, cu_q, cu_kv, kv_len, key_mask, scale, max_q, max_kv)
     on = q.device
     out = torch.empty(a.rows_q, a.ldo, device=on, dtype=q.dtype)
     lse = torch.empty(a.heads, a.rows_q, device=on, dtype=torch.float32)
@@ -998,7 +1006,7 @@ def xattn_bwd(q, k, v, out, dout, lse, heads, *, kv_heads=None, batch=None, cu_q
         with torch.cuda.device(dev):
             return xattn_bwd(q, k, v, out, dout, lse, heads, kv_heads=kv_heads, batch=batch, cu_q=cu_q, cu_kv=cu_kv, kv_len=kv_len, key_mask=key_mask, scale=scale,
                              max_q=max_q, max_kv=max_kv)
-    a, need = _xattn_call(q, k, v, heads, kv_heads, batch, cu_q, cu_kv, kv_len, key_mask, scale, max_q, max_kv)
+    a, need = _xattn_call(dev, q, k, v, heads, kv_heads, batch, cu_q, cu_kv, kv_len, key_mask, scale, max_q, max_kv)
     if not (out.shape == q.shape == dout.shape and out.dtype == q.dtype == dout.dtype):
         raise L.DeclipHipError("bad argument: out and dout like q")
     if lse.shape != (a.heads, a.rows_q) or lse.dtype is not torch.float32 or not lse.is_contiguous():
@@ -1016,7 +1024,7 @@ def xattn_bwd(q, k, v, out, dout, lse, heads, *, kv_heads=None, batch=None, cu_q
 
 
 def _rope_plan(x, pos, heads, sections, theta, joint, interleaved):
-    _req(x.dim() == 2 and heads > 0 and x.shape[1] % heads == 0 and x.shape[1] > 0, "x [rows, heads * hd]")
+    _req(x.dim() == 2 and heads > 0 and x.shape[1] % heads == 0 and x.shape[1] > 0 and x.shape[0] < 1 << 30 and x.shape[1] < 1 << 27, "x [rows, heads * hd], rows below 2^30")
     _row_stride(x, "x")
     dt(x)
     _req(pos.dim() == 2 and pos.shape[1] == len(sections) and pos.dtype in (torch.int32, torch.float32), "pos: contiguous int32 / fp32 [rows, axes]")
@@ -1037,9 +1045,10 @@ def rope_axes(x, pos, heads, sections, theta=10000.0, *, joint=False, interleave
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return rope_axes(x, pos, heads, sections, theta, joint=joint, interleaved=interleaved, inverse=inverse, out=out)
-    sections = tuple(sections)
-    theta = tuple(theta) if isinstance(theta, (tuple, list)) else theta
-    key = ("rope", x.dtype, x.shape, x.stride(), pos.dtype, pos.shape, heads, sections, theta, joint, interleaved)
+    heads, sections = int(heads), tuple(map(int, sections))
+    theta = tuple(map(float, theta)) if isinstance(theta, (tuple, list)) else float(theta)
+    joint, interleaved, inverse = bool(joint), bool(interleaved), bool(inverse)
+    key = ("rope", dev, x.dtype, x.shape, x.stride(), pos.dtype, pos.shape, heads, sections, theta, joint, interleaved)
     plan, d, rows, width, pos_rows, frac = _plan(key, lambda: _rope_plan(x, pos, heads, sections, theta, joint, interleaved))
     if not pos.is_contiguous():
         raise L.DeclipHipError("bad argument: pos: contiguous int32 / fp32 [rows, axes]")
@@ -1059,20 +1068,29 @@ JoinNormGrads = collections.namedtuple("JoinNormGrads", "post_w post_b gate scal
 
 
 def _join_plan(x, y, gate, rms, gate_tanh, alpha, eps):
-    _req(x.dim() == 2 and x.shape == y.shape and x.dtype == y.dtype, "x and y [rows, d] of one dtype")
+    _req(x.dim() == 2 and x.shape == y.shape and x.dtype == y.dtype and max(x.shape) < 1 << 30, "x and y [rows, d] of one dtype, rows below 2^30")
     a = L.JoinNormArgs()
-    a.dtype, a.rms, a.gate_tanh, a.alpha, a.eps = dt(x), int(rms), int(gate_tanh), float(alpha), float(eps)
+    a.dtype, a.rms, a.gate_tanh, a.alpha, a.eps = dt(x), rms, gate_tanh, alpha, eps
     a.rows, a.d = x.shape
     if gate is not None:
         _req(gate.dtype == torch.float32 and gate.dim() <= 2 and (gate.dim() < 2 or gate.shape[1] == a.d), "gate: contiguous fp32 [groups] or [groups, d]")
         a.gate_rows, a.gate_channel = (gate.shape[0] if gate.dim() else 1), int(gate.dim() == 2)
         _req(a.gate_rows > 0 and a.rows % a.gate_rows == 0, "gate: %d groups of %d rows" % (a.gate_rows, a.rows))
-    return a
+    # (the backward's workspace depends on sizes, not on places: any address will do)
+    probe = L.JoinNormArgs.from_buffer_copy(a)
+    probe.x = probe.y = probe.stats = 16
+    probe.gate = None if gate is None else 16
+    need = L.load().dh_join_norm_bwd_ws_bytes(ctypes.byref(probe))
+    if need < 0:
+        check(-1, "dh_join_norm")
+    return a, need
 
 
-def _join_call(x, y, post, gate, scale, pre, alpha, eps, rms, gate_tanh):
-    key = ("join", x.dtype, x.shape, y.dtype, y.shape, None if gate is None else (gate.dtype, gate.shape), rms, gate_tanh, alpha, eps)
-    a = L.JoinNormArgs.from_buffer_copy(_plan(key, lambda: _join_plan(x, y, gate, rms, gate_tanh, alpha, eps)))
+def _join_call(dev, x, y, post, gate, scale, pre, alpha, eps, rms, gate_tanh):
+    rms, gate_tanh, alpha, eps = bool(rms), bool(gate_tanh), float(alpha), float(eps)
+    key = ("join", dev, x.dtype, x.shape, y.dtype, y.shape, None if gate is None else (gate.dtype, gate.shape), rms, gate_tanh, alpha, eps)
+    plan, need = _plan(key, lambda: _join_plan(x, y, gate, rms, gate_tanh, alpha, eps))
+    a = L.JoinNormArgs.from_buffer_copy(plan)
     d = a.d
     if not (x.is_contiguous() and y.is_contiguous() and (gate is None or gate.is_contiguous())):
         raise L.DeclipHipError("x, y and gate must be contiguous")
@@ -1094,7 +1112,7 @@ def _join_call(x, y, post, gate, scale, pre, alpha, eps, rms, gate_tanh):
         a.scale = vec(scale, "scale")
     if gate is not None:
         a.gate = gate.data_ptr()
-    return a
+    return a, need
 
 
 def join_norm_fwd(x, y, *, post=None, gate=None, scale=None, pre=None, alpha=1.0, eps=1e-5, rms=False, gate_tanh=False):
@@ -1106,7 +1124,7 @@ def join_norm_fwd(x, y, *, post=None, gate=None, scale=None, pre=None, alpha=1.0
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return join_norm_fwd(x, y, post=post, gate=gate, scale=scale, pre=pre, alpha=alpha, eps=eps, rms=rms, gate_tanh=gate_tanh)
-    a = _join_call(x, y, post, gate, scale, pre, alpha, eps, rms, gate_tanh)
+    a, _ = _join_call(dev, x, y, post, gate, scale, pre, alpha, eps, rms, gate_tanh)
     x_out, n = torch.empty_like(x), None if pre is None else torch.empty_like(x)
     stats = torch.empty(4, a.rows, device=x.device, dtype=torch.float32)
     a.x_out, a.stats = x_out.data_ptr(), stats.data_ptr()
@@ -1125,7 +1143,7 @@ def join_norm_bwd(x, y, dx_out, dn, stats, *, post=None, gate=None, scale=None, 
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return join_norm_bwd(x, y, dx_out, dn, stats, post=post, gate=gate, scale=scale, pre=pre, alpha=alpha, eps=eps, rms=rms, gate_tanh=gate_tanh)
-    a = _join_call(x, y, post, gate, scale, pre, alpha, eps, rms, gate_tanh)
+    a, need = _join_call(dev, x, y, post, gate, scale, pre, alpha, eps, rms, gate_tanh)
     for t, name in ((dx_out, "dx_out"), (dn, "dn")):
         if t is not None and not (t.shape == x.shape and t.dtype is x.dtype and t.is_contiguous()):
             raise L.DeclipHipError("bad argument: %s: like x, contiguous" % name)
@@ -1138,9 +1156,7 @@ def join_norm_bwd(x, y, dx_out, dn, stats, *, post=None, gate=None, scale=None, 
     a.dx_out, a.dn = None if dx_out is None else dx_out.data_ptr(), None if dn is None else dn.data_ptr()
     a.stats, a.dx, a.dy = stats.data_ptr(), dx.data_ptr(), dy.data_ptr()
     a.d_post_w, a.d_post_b, a.d_gate, a.d_scale, a.d_pre_w, a.d_pre_b = (None if t is None else t.data_ptr() for t in grads)
-    lib = L.load()
-    need = lib.dh_join_norm_bwd_ws_bytes(ctypes.byref(a))
     ws = torch.empty(max(need, 16) // 4, device=x.device, dtype=torch.float32)
     a.ws, a.ws_bytes = ws.data_ptr(), need
-    check(lib.dh_join_norm_bwd(ctypes.byref(a), _stream_on(dev)), "dh_join_norm_bwd")
+    check(L.load().dh_join_norm_bwd(ctypes.byref(a), _stream_on(dev)), "dh_join_norm_bwd")
     return dx, dy, grads

@@ -23,6 +23,10 @@ CASES = ([("test_xattn", (dt,) + c) for dt in (BF16, F32) for c in [
              (9, 2056, 3, "row", True, True, False, True, True, False, 0.5), (6, 5000, 2, "channel", True, False, True, True, True, True, 1.0),
              (14, 33, 7, "row", False, True, True, True, True, False, 1.0), (5, 257, 1, "channel", False, False, True, False, True, False, 1.0),
              (4, 3001, 4, "row", False, False, False, True, True, True, 1.0), (6, 1, 2, "row", False, True, False, True, False, False, 1.0)]]
+         + [("test_xattn_block_shapes_and_split_axes", (BF16,) + c) for c in [
+             (2, 2, 64, 1, 300, 20, False, 0.2), (1, 1, 128, 1, 33, 40, True, 0.0), (1, 1, 128, 1, 130, 140, True, 0.1), (1, 1, 64, 1, 130, 2050, True, 0.0), (1, 1, 96, 1, 130, 300, False, 0.0)]]
+         + [("test_join_norm_rows_far_from_zero", (dt, rms)) for dt in (BF16, F32) for rms in (False, True)]
+         + [("test_gradients_that_arrive_expanded_or_far_apart", ()), ("test_numbers_given_as_tensors_are_read_on_every_call", ())]
          + [("test_join_norm_one_gradient_only", (w,)) for w in ("dn", "dx_out")] + [("test_join_norm_no_rows", ())]
          + [("test_gated_cross_attention_blocks_and_their_gradients", (dt,)) for dt in (F32, BF16)] + [("test_finite_differences", ())])
 
@@ -72,6 +76,10 @@ def test_xattn_refusals():
         _refused(lambda: f(q.t(), k, k, 1, batch=1), "contiguous columns")
         _refused(lambda: f(z(4, 131)[:, 3:], k, k, 2, batch=1), "16-byte")
         _refused(lambda: f(q, z(1, 128).expand(6, 128), k, 2, batch=1), "16-byte")
+        far = z((1 << 22) + 128).as_strided((2, 128), (1 << 22, 1))
+        _refused(lambda: f(q, far, far, 2, batch=1), "2^22")
+        many = z(1).expand(1 << 30, 8)
+        _refused(lambda: f(many, z(6, 8), z(6, 8), 1, batch=1), "2^30")
         out, lse = f(q, k, k, 2, batch=1)
         b = ops.xattn_bwd
         _refused(lambda: b(q, k, k, out, out[:3], lse, 2, batch=1), "dout")
@@ -98,6 +106,7 @@ def test_rope_refusals():
         _refused(lambda: f(x.half(), pos, 2, (4, 4)), "dtype")
         _refused(lambda: f(x.t(), pos, 2, (4, 4)), "contiguous columns")
         _refused(lambda: f(x, pos, 2, (4, 4), out=x[:5]), "out")
+        _refused(lambda: f(x[:1, :1].expand(1 << 30, 8), pos, 1, (4,)), "2^30")
         wide = torch.zeros(7, 128, dtype=BF16)
         _refused(lambda: f(wide[:6], pos, 2, (4, 4), out=wide[1:]), "out")
 
@@ -118,6 +127,8 @@ def test_join_norm_refusals():
         _refused(lambda: f(x, x, gate=torch.ones(2, 3)), "gate")
         _refused(lambda: f(x, x, gate=torch.ones(0)), "groups")
         _refused(lambda: f(x, x, eps=-1.0), "eps")
+        many = x[:1, :1].expand(1 << 30, 8)
+        _refused(lambda: f(many, many), "2^30")
         _refused(lambda: f(torch.zeros(2, 8200), torch.zeros(2, 8200)), "8192")
         _refused(lambda: f(torch.zeros(2, 0), torch.zeros(2, 0)), "width 0")
         _, n, st = f(x, x, pre=(w, None))

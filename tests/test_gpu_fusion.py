@@ -122,6 +122,35 @@ def test_xattn_single_tokens_over_long_keys(dtype, heads, kv_heads, hd, b, lq, s
     xattn_case(dtype, heads, kv_heads, hd, *geometry(b, lq, s, True, seed=s), grads=False)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads,kv_heads,hd,b,lq,s,packed,mask", [
+    (2, 2, 64, 1, 600, 50, False, 0.2), (2, 1, 64, 2, 700, 40, True, 0.0), (2, 2, 128, 3, 77, 100, True, 0.0), (2, 1, 128, 2, 200, 300, True, 0.1), (3, 3, 96, 2, 150, 260, False, 0.0),
+    (1, 1, 128, 1, 300, 1500, False, 0.3), (2, 2, 64, 1, 150, 2100, True, 0.0), (4, 1, 64, 1, 70, 3100, False, 0.1), (2, 2, 32, 2, 900, 300, True, 0.0), (2, 2, 72, 1, 129, 700, False, 0.0)])
+def test_xattn_block_shapes_and_split_axes(dtype, heads, kv_heads, hd, b, lq, s, packed, mask):
+    """1 to 8 waves per block, the other axis whole and in ranges, for each of the three kernels"""
+    xattn_case(dtype, heads, kv_heads, hd, *geometry(b, lq, s, packed, seed=lq + s), mask=mask)
+
+
+def test_xattn_rows_far_apart():
+    """element offsets beyond 2^31: the rows of a long cache, 2^21 elements apart"""
+    ops = _ops()
+    rows_q, rows_kv, ld, w = 1040, 1100, 1 << 21, 128
+    q, k, v, dout = (rnd(n, w, seed=i, dtype=BF16) for i, n in enumerate((rows_q, rows_kv, rows_kv, rows_q)))
+    ref = R.xattn(q, k, v, 2, dout, batch=1)
+    cache = torch.empty(rows_kv, ld, dtype=BF16, device=cuda)
+    cache[:, 256:256 + w], cache[:, ld - w:] = k.to(cuda), v.to(cuda)
+    far = torch.empty(rows_q, ld, dtype=BF16, device=cuda)
+    far[:, 8:8 + w], far[:, 512:512 + w] = q.to(cuda), dout.to(cuda)
+    qd, dd, kd, vd = far[:, 8:8 + w], far[:, 512:512 + w], cache[:, 256:256 + w], cache[:, ld - w:]
+    out, lse = ops.xattn_fwd(qd, kd, vd, 2, batch=1)
+    check(out, *ref["out"], "out")
+    for name, t in zip(("dq", "dk", "dv"), ops.xattn_bwd(qd, kd, vd, out, dd, lse, 2, batch=1)):
+        check(t, *ref[name], name)
+    pos = torch.arange(rows_q, dtype=torch.int32)[:, None].contiguous()
+    y = ops.rope_axes(qd, pos.to(cuda), 2, (32,))
+    check(y, *R.rope(q, pos, 2, (32,)), "rope")
+
+
 def test_xattn_split_ranges_without_a_key():
     """whole ranges of the split key axis are masked, one sequence has nothing but masked keys"""
     ops = _ops()
@@ -306,6 +335,36 @@ def test_join_norm_unaligned_rows_and_same_bits():
             assert torch.equal(s, t)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rms", [False, True])
+def test_join_norm_rows_far_from_zero(dtype, rms):
+    """rows whose mean is a thousand times their deviation, and rows of one value (their deviation is eps's)"""
+    xy, kw = join_inputs(dtype, 40, 520, 4, "row", True, True, True, True, rms)
+    far = torch.linspace(-2000, 2000, 40)[:, None]
+    xy = {n: (t.float() + far).to(dtype) for n, t in xy.items()}
+    xy["y"][7] = 3.0
+    xy["x"][9], xy["y"][9] = 0.0, -0.0
+    join_check(dtype, xy, kw, dict(rms=rms), rnd(40, 520, seed=20, dtype=dtype), rnd(40, 520, seed=21, dtype=dtype))
+
+
+def test_join_norm_more_elements_than_31_bits():
+    ops = _ops()
+    rows, d = (1 << 18) + 3, 8192
+    xy, kw = join_inputs(BF16, 4, d, 1, "row", True, True, True, True, False)
+    some = torch.tensor([0, 1, rows - 2, rows - 1], device=cuda)
+    full = {n: torch.zeros(rows, d, dtype=BF16, device=cuda).index_copy_(0, some, t.to(cuda)) for n, t in xy.items()}
+    g = rnd(4, d, seed=20, dtype=BF16)
+    gd = torch.zeros(rows, d, dtype=BF16, device=cuda).index_copy_(0, some, g.to(cuda))
+    ref = R.join(**xy, **kw, dx_out=g, dn=g)
+    tol = R.join_bounds(ref, **xy, **kw, dx_out=g, dn=g)
+    x_out, n, stats = ops.join_norm_fwd(**full, **on_gpu(kw))
+    dx, dy, grads = ops.join_norm_bwd(full["x"], full["y"], gd, gd, stats, **on_gpu(kw))
+    for name, t in dict(x_out=x_out, n=n, dx=dx, dy=dy).items():
+        check(t[some], ref[name], tol[name], name)
+    for name in ("post_w", "pre_w", "gate", "scale"):        # (rows without a gradient add zeros)
+        check(getattr(grads, name), ref[name], tol[name], name)
+
+
 def test_join_norm_no_rows():
     ops = _ops()
     xy, kw = join_inputs(F32, 0, 64, 1, "none", True, True, True, True, False)
@@ -396,6 +455,42 @@ def test_gated_cross_attention_blocks_and_their_gradients(dtype):
     tol = 2000 * R.UF if dtype == F32 else 2 * math.sqrt(30) * R.UB
     for n, a, b in zip(names, *results):
         assert float((a - b).norm()) <= tol * (sums.pop(0) if n == "gate" else float(a.norm())), n
+
+
+def test_gradients_that_arrive_expanded_or_far_apart():
+    """the gradient of a sum is one element seen everywhere; rows may come with any stride"""
+    from declip_amd import fusion
+    q, k, v = (rnd(n, 64, seed=i).to(cuda) for i, n in enumerate((6, 10, 10)))
+    pos = torch.arange(6, dtype=torch.int32, device=cuda)[:, None].contiguous()
+    w = torch.ones(64, device=cuda)
+
+    def grads(out_of, *leaves):
+        leaves = [t.clone().requires_grad_(True) for t in leaves]
+        outs = out_of(*leaves)
+        ones = torch.autograd.grad([o.sum() for o in outs], leaves)
+        return ones, torch.autograd.grad(out_of(*leaves), leaves, [torch.ones_like(o) for o in outs])
+
+    for a, b in (grads(lambda *t: (fusion.cross_attention(*t, 2, batch=2),), q, k, v), grads(lambda t: (fusion.rope_axes(t, pos, 2, (16,)),), q),
+                 grads(lambda x, y: fusion.join_norm(x, y, post=(w, None), pre=(w, None)), q, q * 2)):
+        for s, t in zip(a, b):
+            assert torch.equal(s, t)
+    apart = torch.zeros(10 * (1 << 22) + 64, device=cuda).as_strided((10, 64), (1 << 22, 1))
+    apart.copy_(k)
+    assert torch.equal(fusion.cross_attention(q, apart, v, 2, batch=2), fusion.cross_attention(q, k, v, 2, batch=2))
+
+
+def test_numbers_given_as_tensors_are_read_on_every_call():
+    ops = _ops()
+    q, k = rnd(6, 64, seed=1).to(cuda), rnd(10, 64, seed=2).to(cuda)
+    scale, most = torch.tensor(0.5, device=cuda), torch.tensor(3, device=cuda)
+    first = ops.xattn_fwd(q, k, k, 2, batch=2, scale=scale, max_q=most)[0]
+    scale.fill_(0.125)
+    second = ops.xattn_fwd(q, k, k, 2, batch=2, scale=scale, max_q=most)[0]
+    assert torch.equal(first, ops.xattn_fwd(q, k, k, 2, batch=2, scale=0.5)[0]) and torch.equal(second, ops.xattn_fwd(q, k, k, 2, batch=2, scale=0.125)[0])
+    alpha = torch.tensor(2.0)
+    first = ops.join_norm_fwd(q, q, alpha=alpha)[0]
+    alpha.fill_(3.0)
+    assert torch.equal(first, 3 * q) and torch.equal(ops.join_norm_fwd(q, q, alpha=alpha)[0], 4 * q)
 
 
 def test_finite_differences():
