@@ -9,9 +9,11 @@
 //   C[c] = sum dn xhat = dpre_w, E[c] = sum dn = dpre_b;   dgate = the same sums per group (channel gate) or sum_c G scale p (row gate)
 //
 // HBM-bound: the forward reads x, y and writes x', n; the backward reads x, y, dx', dn, recomputes p, x', xhat from the rows' saved statistics
-// (in fp32, the forward's own values) and writes dx, dy.  A row lives in the registers of one wave (d <= 1024) or of one block, statistics
+// (in fp32, the forward's own values) and writes dx, dy.  A row lives in the registers of 1 to 8 waves, statistics
 // are fp32 and two-pass (mean first).  The column sums stay in registers over a block's rows, go to a partial row per block, and are
 // added in a fixed order by a second small kernel: no atomics, the same result on every run.
+// Measured, bf16: 25600 rows of 768, a gate vector per 50 rows: forward 33 us (157 MB: 4.8 TB/s), backward 55 + 8 us (236 MB: 4.2 TB/s); 8191 rows of 4096,
+// one gate: 51 us (268 MB: 5.3 TB/s), 97 + 8 us (403 MB: 4.2 TB/s).
 #include "dh_common.h"
 #include <initializer_list>
 
@@ -508,7 +510,8 @@ __global__ __launch_bounds__(1024) void join_reduce_kernel(JP p, int blocks, int
 struct Shape { int w, nc, v; };
 // 1, 2, 4 or 8 waves per row, so that a lane holds 8 or 12 columns (the backward's four column sums, three parameter vectors, four operands and the
 // next row's fit its registers).  8 elements per access, or 4 where that leaves no lane idle (768 columns: three full accesses instead of one and a
-// half); single elements where the width or an address rules vectors out.
+// half); single elements where the width or an address rules vectors out.  One wave up to 1024 columns and a block above, no row
+// fetched ahead: forward 44 us, backward 86 (25600 x 768), 61 and 130 (8191 x 4096).
 bool shape_of(int d, int vec, Shape& s) {
   const int w = d <= 768 ? 1 : d <= 1536 ? 2 : d <= 2048 ? 4 : 8;
   if (vec == 1) s = d <= 256 ? Shape{1, 4, 1} : d <= 4096 ? Shape{8, 8, 1} : Shape{8, 16, 1};
@@ -544,6 +547,7 @@ int blocks_of(const dh_join_norm_args* a, int w, int most, int& per_group) {
   per_group = dh_cdiv(dh_cdiv(a->rows, n), g) * g;
   return dh_cdiv(a->rows, per_group);
 }
+// one block per compute unit: its column sums leave once (two rounds of blocks at 25600 x 768: 109 us against 55)
 int bwd_blocks(const dh_join_norm_args* a, int w, int& per_group) { return blocks_of(a, w, j_cus(), per_group); }
 
 int check(const dh_join_norm_args* a, const char* who) {

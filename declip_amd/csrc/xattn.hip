@@ -17,6 +17,12 @@
 // bf16: v_mfma_f32_32x32x16_bf16, P and dS rounded to bf16 as MFMA operands (their sums are formed before, in fp32); fp32:
 // v_mfma_f32_32x32x2_f32, nothing rounded.
 //
+// What bounds it, measured (bf16): 256 captions of 5 .. 77 tokens on 197 keys, 8 heads of 64 (mean 41 rows a pair): latency of short blocks, 31 / 35 / 58 us
+// (fwd / dq / dkv; q, k, v, o, do, dq, dk, dv once: 48 us for all three).  16 pairs of 4096 rows on 1568 .. 3136 keys, hd 128: 140 us (105 GFLOP at full length),
+// dq 180, dkv 295: products, exponentials and LDS reads of a tile take about the same time and overlap by half.
+// 24 pairs of 2047 rows on 6272 keys, hd 64: 102 + 9 us = 700 TFLOP/s, the exponentials alone take 103 us at the full vector rate.  64 sequences of one token, 4 kv heads,
+// up to 3136 keys: 27 + 7 us, 129 MB = 4.8 TB/s.  fp32: 64-cycle instructions in a chain, 16 sequences of up to 77 on 257, 12 heads of 80: 40 / 50 / 44 us.
+//
 // Keys outside the sequence or masked: their rows are staged as ZEROS (whatever the memory holds, NaN included) and their scores are
 // -inf.  A row without a valid key: o = 0, lse = -inf, no gradient.  Rows that no sequence owns are written as zeros (lse -inf).
 #include "dh_common.h"
@@ -214,6 +220,15 @@ __device__ __forceinline__ void load_row(typename Op<T>::Frag* f, const T* row, 
     if (live && c < hd) x.u = *reinterpret_cast<const uint4*>(row + c);
     f[ks] = x.f;
   }
+}
+// The operand rows are here: a use in front of the tile loop, on every path to it.  Without it the compiler places their wait at the loop's first
+// product, where it waits on every turn for ALL loads under way, the next tile's too.
+template <typename F, int KS>
+__device__ __forceinline__ void arrived(F (&f)[KS]) {
+#ifndef DH_HOST_EMU
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(f[ks]));
+#endif
 }
 template <typename T, int HDP>
 __device__ __forceinline__ f32x16_t mma_row(const T* tile, int row0, const typename Op<T>::Frag* f, int lane) {
@@ -686,6 +701,14 @@ __global__ __launch_bounds__(64 * RW, (waves_dq<T, HDP, RW>())) void xattn_dq_ke
   }
 }
 
+// a value the compiler knows nothing about: what follows from it is computed again where it is used
+__device__ __forceinline__ int opaque(int v) {
+#ifndef DH_HOST_EMU
+  asm volatile("" : "+v"(v));
+#endif
+  return v;
+}
+
 // ------------------------------------------------------------------------------------------ backward: dk, dv
 template <typename T, int HDP, int RW, bool SPLIT>
 __global__ __launch_bounds__(64 * RW, (waves_dkv<T, HDP, RW>())) void xattn_dkv_kernel(XP p) {
@@ -722,7 +745,7 @@ __global__ __launch_bounds__(64 * RW, (waves_dkv<T, HDP, RW>())) void xattn_dkv_
       for (int i = 0; i < 16; ++i) dk[d][i] = dv[d][i] = 0.f;
     Pair2<T, HDP, BQ, NT> st;
     float nlse = 0.f, ndel = 0.f;
-    auto fetch = [&](int mt) {
+    auto fetch = [&](int mt, int tid) {
       const int m0 = mt * BQ;
       int q0, r0;
       m_split(p, m0, q0, r0);                          // (uniform: the tile's first row)
@@ -735,7 +758,7 @@ __global__ __launch_bounds__(64 * RW, (waves_dkv<T, HDP, RW>())) void xattn_dkv_
         ndel = p.delta[stat];
       }
     };
-    auto store = [&](int mt) {
+    auto store = [&](int mt, int tid) {
       T* b = buf + (mt & 1) * 2 * BQ * LD;
       st.store(b, b + BQ * LD, (mt + 1) * BQ > M || p.hd < HDP, mt * BQ, M - 1, false, p.hd, tid);
       if (tid < BQ) {
@@ -746,15 +769,18 @@ __global__ __launch_bounds__(64 * RW, (waves_dkv<T, HDP, RW>())) void xattn_dkv_
     };
     const int hi_mt = block_live ? hi : lo;
     if (lo < hi_mt) {
-      fetch(lo);
-      store(lo);
-      if (lo + 1 < hi_mt) fetch(lo + 1);
-      __syncthreads();
+      fetch(lo, tid);
+      store(lo, tid);
     }
+    if constexpr (sizeof(T) == 2) { arrived(kf); arrived(vf); }      // (fp32, with accumulation registers to spare, is 3 % slower with it)
+    if (lo + 1 < hi_mt) fetch(lo + 1, tid);
+    if (lo < hi_mt) __syncthreads();
     for (int mt = lo; mt < hi_mt; ++mt) {
+      // (a thread's places in the tiles are formed anew on every turn: kept, they are spilled, and a reload waits for all loads under way)
+      const int tid = opaque(threadIdx.x), lane = tid & 63, h = lane >> 5;
       if (mt + 1 < hi_mt) {
-        store(mt + 1);
-        if (mt + 2 < hi_mt) fetch(mt + 2);
+        store(mt + 1, tid);
+        if (mt + 2 < hi_mt) fetch(mt + 2, tid);
       }
       if (wave_live) {
         const T *Qs = buf + (mt & 1) * 2 * BQ * LD, *Ds = Qs + BQ * LD;
