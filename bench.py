@@ -255,11 +255,16 @@ def _arm_watchdog(seconds, what):
     """Last line of defence for the DEFAULT multi-GPU configuration (captured step with RCCL collectives in the graph), which has
     never run on more than one rank: if `what` makes no progress for `seconds`, this rank re-executes itself with --graph 0.  A hang
     inside a collective stops every rank, so every rank's watchdog fires and the re-executed ranks meet again in a fresh rendezvous
-    (torchrun: the agent's store with the next attempt prefix; self-launched: the next port).  exec closes the device files, so
-    the driver tears down the hung queues of the old image.  The line then carries `graph_fallback`.  Returns the timer (cancel())."""
+    (torchrun: the agent's store with the next attempt prefix; self-launched: the next port).  The new attempt is a child process -- a
+    program that has initialised the GPU must not exec -- whose exit code becomes this rank's; this process does nothing more but wait
+    for it (its queues, hung or not, go when it ends).  The line then carries `graph_fallback`.  Returns the timer (cancel())."""
+    import subprocess
     import threading
 
+    fired = threading.Event()
+
     def fire(msg=None):
+        fired.set()
         msg = msg or "watchdog: %s made no progress in %d s; rank re-executed with --graph 0" % (what, int(seconds))
         sys.stderr.write("bench.py: " + msg + "\n")
         sys.stderr.flush()
@@ -279,14 +284,18 @@ def _arm_watchdog(seconds, what):
             if a.startswith("--graph="):
                 continue
             argv.append(a)
-        # (no closing of other descriptors here: helper threads of the runtime abort the process when their sockets vanish under
-        # them, before exec gets to run -- seen on the MI355X.  The device files are opened O_CLOEXEC by the ROCm runtime, so exec
-        # itself releases the hung queues; sockets of the old rendezvous that survive are harmless, the new one uses another port.)
-        if _JSON_FD is not None:
-            os.dup2(_JSON_FD, 1)                  # the new image claims the real stdout again
-        os.execve(sys.executable, [sys.executable, os.path.abspath(__file__)] + argv + ["--graph", "0"], env)
+        # (the old rendezvous' sockets stay with this process: the new one uses another port)
+        code = subprocess.call([sys.executable, os.path.abspath(__file__)] + argv + ["--graph", "0"], env=env, stdout=_JSON_FD)      # None: stdout as it is
+        os._exit(code if code >= 0 else 128 - code)
     t = threading.Timer(seconds, fire)
     t.daemon = True
+    stop = t.cancel
+
+    def cancel():
+        stop()
+        if fired.is_set():
+            t.join()          # (the step came back after all, too late: the new attempt speaks for this rank, and ends it)
+    t.cancel = cancel
     t.reexec = fire           # the same way out for a captured step that RAISES (GraphedStep: invalidated capture / failed first launch)
     t.start()
     return t
