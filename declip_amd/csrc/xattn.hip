@@ -19,7 +19,7 @@
 //
 // What bounds it, measured (bf16): 256 captions of 5 .. 77 tokens on 197 keys, 8 heads of 64 (mean 41 rows a pair): latency of short blocks, 31 / 35 / 58 us
 // (fwd / dq / dkv; q, k, v, o, do, dq, dk, dv once: 48 us for all three).  16 pairs of 4096 rows on 1568 .. 3136 keys, hd 128: 140 us (105 GFLOP at full length),
-// dq 180, dkv 295: products, exponentials and LDS reads of a tile take about the same time and overlap by half.
+// dq 180, dkv 270-295: products, exponentials and LDS reads of a tile take about the same time and overlap by half.
 // 24 pairs of 2047 rows on 6272 keys, hd 64: 102 + 9 us = 700 TFLOP/s, the exponentials alone take 103 us at the full vector rate.  64 sequences of one token, 4 kv heads,
 // up to 3136 keys: 27 + 7 us, 129 MB = 4.8 TB/s.  fp32: 64-cycle instructions in a chain, 16 sequences of up to 77 on 257, 12 heads of 80: 40 / 50 / 44 us.
 //
@@ -852,7 +852,7 @@ enum Kind { FWD, DQ, DKV };
 // on 197 keys fwd 31 / 39 / 42, dq 36 / 52 / 48, dkv 58 / 60 / 62; 197 rows on 5 .. 77 keys fwd 42 / 37 / 48, dq 58 / 65 / 72; 128 pairs of 512 on 512 fwd
 // 26 / 23 / 18, dkv 39 / 32 / 29; 24 pairs of 2047 on 6272 fwd 226 / 198 / 147.
 // More than 64 columns: eight waves (half of the staging registers each, two waves per SIMD) once they are filled: 16 pairs of 4096 rows on 3136 keys fwd
-// 164 (four: 170), dq 191 (319), dkv 382 (612).  fp32 is bound by its matrix instructions: four.
+// 164 (four: 170), dq 191 (319), dkv 382 (612; both before the padding and the spill-free loop below).  fp32 is bound by its matrix instructions: four.
 int row_waves(const dh_xattn_args* a, Kind kind, int64_t rows, int64_t other) {
   if (rows <= 32) return 1;
   if (a->dtype == DH_F32) return 4;

@@ -193,7 +193,8 @@ int dh_attn_pooled_bwd(int dtype, const void* q, const void* kv, const void* dou
  * tokens; the reference declares such a branch, return_caption of model/declip.py:166-167, and never builds it):
  *   s = scale q k^T over the valid keys, p = softmax(s), out = p v, lse = log sum exp s
  * Layout: token-major rows, head-major columns.  q / out / dout / dq [rows_q][heads*hd], k / v / dk / dv [rows_kv][kv_heads*hd], each with its own
- * row stride in elements (k and v may be the halves of one [rows][2*kv_heads*hd] projection), 16-byte aligned rows; lse [heads][rows_q] fp32.
+ * row stride in elements, below 2^22 (k and v may be the halves of one [rows][2*kv_heads*hd] projection), 16-byte aligned rows; lse [heads][rows_q]
+ * fp32.  rows_q * (heads / kv_heads) and rows_kv below 2^30.
  *   heads % kv_heads == 0: query head h reads kv head h / (heads / kv_heads) and dk / dv are summed over it.  hd: a multiple of 8 up to 128.
  *   Sequence i owns query rows cu_q[i] .. cu_q[i+1] and key rows cu_kv[i] .. cu_kv[i+1] (int32 [batch + 1], device memory, ascending); a NULL
  *   table means rows / batch rows each.  kv_len (int32 [batch], or NULL): only the first kv_len[i] of them are keys.  key_mask (1 byte per key
@@ -227,7 +228,7 @@ int dh_xattn_bwd(const dh_xattn_args* args, dh_stream_t stream);
 /* ---------------------------------------------------------------- rotary positions ------
  * Rotary positions with several axes (time, height, width of image / video tokens) on `heads` heads of hd columns each; beside the learned
  * tables of image_encoder/visual_transformer.py:20-22 and text_encoder/text_transformer.py:99.  x [rows][>= heads*hd] (row stride ldx; e.g. the q
- * and k columns of a fused projection as 2*heads heads), y likewise, y == x allowed (in place), otherwise disjoint.
+ * and k columns of a fused projection as 2*heads heads; rows < 2^30), y likewise, y == x allowed (in place), otherwise disjoint.
  * Axis a turns sections[a] pairs, in the order of the axes; P = their sum, 2 P <= hd, P <= 128; columns behind 2 P of a head are copied.
  *   pair i = columns (i, P + i), interleaved: (2 i, 2 i + 1) of a head
  *   angle  = pos[row % pos_rows][axis] * theta[axis] ^ (-j / sections[axis]), j = the pair's place in its axis (joint: theta ^ (-i / P))
@@ -251,7 +252,7 @@ int dh_rope_axes(const dh_rope_plan* plan, int dtype, const void* x, int64_t ldx
  *   N: LayerNorm (z - mean) rstd w + b (b may be NULL), or RMS norm z rstd w (rms = 1); fp32 parameters [d]
  *   g: 1 (gate NULL) or gate (gate_tanh: tanh(gate)), fp32, one value per rows / gate_rows consecutive rows ([gate_rows]) or one
  *   vector ([gate_rows][d], gate_channel = 1)
- * x, y, x_out, n, dx_out, dn, dx, dy [rows][d] contiguous, d <= 8192; 16-byte accesses where d % 8 == 0 and the addresses allow it.
+ * x, y, x_out, n, dx_out, dn, dx, dy [rows][d] contiguous, rows < 2^30, d <= 8192, gate vectors < 2^22; 16-byte accesses where d % 8 == 0 and the addresses allow it.
  * stats [4][rows] fp32: mean / rstd of both norms, written by fwd, read by bwd.  n is computed from x_out before its rounding to dtype.
  * bwd: dx_out and dn are the gradients of the two outputs (one may be NULL); parameter gradients are WRITTEN (not accumulated), fp32, NULL =
  * not wanted; ws: dh_join_norm_bwd_ws_bytes(args).  No atomics: the same bits on every run. */
