@@ -24,11 +24,15 @@ FAST_MATH = ["-ffast-math", "-fno-finite-math-only"]
 # The cross-tower operators (xattn / rope / join_norm) are IEEE as well: their bound is memory or the matrix units, and a reassociated sum would only
 # move their results away from the formulas.
 IEEE_SOURCES = {"filip.hip", "declip_ops.hip", "xattn.hip", "rope.hip", "join_norm.hip"}
+# LayerNorm's sums keep the order the source gives them: without packed fp32 the compiler pairs them differently, and the two-rank DeFILIP step, whose
+# BatchNorm heads divide by the spread of a handful of rows, leaves its 1e-3 gate by that alone (22.62 ms per CLIP step either way)
+ORDERED_SOURCES = {"layernorm.hip"}
 FLAGS = BASE_FLAGS + FAST_MATH                 # (the digest below covers both variants)
 
 
 def flags_for(src):
-    return BASE_FLAGS + ([] if os.path.basename(src) in IEEE_SOURCES else FAST_MATH)
+    name = os.path.basename(src)
+    return BASE_FLAGS + ([] if name in IEEE_SOURCES else FAST_MATH + (["-fno-associative-math"] if name in ORDERED_SOURCES else []))
 
 
 def sources():
@@ -36,7 +40,7 @@ def sources():
 
 
 def _digest():
-    h = hashlib.sha256((" ".join(FLAGS) + "|ieee:" + ",".join(sorted(IEEE_SOURCES))).encode())
+    h = hashlib.sha256((" ".join(FLAGS) + "|ieee:" + ",".join(sorted(IEEE_SOURCES)) + "|ordered:" + ",".join(sorted(ORDERED_SOURCES))).encode())
     files = sources() + [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith(".h")]
     files.append(os.path.join(os.path.dirname(HERE), "include", "declip_hip.h"))
     for f in files:
