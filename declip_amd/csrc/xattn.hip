@@ -12,14 +12,15 @@
 // (key 8i + 4h + r <-> slot (h, 4i' + r)), V^T's fragment is read from the row-major tile by the transpose read with the same numbering.
 // P never leaves the registers.
 //   fwd   a wave owns 32 rows m, Q in registers, K / V tiles in LDS
-//   dq    the same with dO in registers too: dP^T = V dO^T, dS^T, dQ^T += K^T dS^T;  writes D for dkv
+//   dq    the same with dO in registers too: dP^T = V dO^T, D = sum p dp, then dS^T, dQ^T += K^T dS^T;  writes D for dkv
 //   dkv   a wave owns 32 keys, K / V in registers, Q / dO tiles in LDS: S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS
-// bf16: v_mfma_f32_32x32x16_bf16, P and dS rounded to bf16 as MFMA operands (their sums are formed before, in fp32); fp32:
-// v_mfma_f32_32x32x2_f32, nothing rounded.
+// bf16: v_mfma_f32_32x32x16_bf16.  P and dS are rounded to bf16 as its operands, the one rounding between inputs and results: independent element by element,
+// it costs the results about as much as their own rounding (1.7e-3 of the norm each), and kept in two bf16 parts P and dS would double half of the
+// products.  Their sums (l, D) are formed before, in fp32.  fp32: v_mfma_f32_32x32x2_f32, nothing rounded.
 //
-// What bounds it, measured (bf16): 256 captions of 5 .. 77 tokens on 197 keys, 8 heads of 64 (mean 41 rows a pair): latency of short blocks, 31 / 35 / 58 us
-// (fwd / dq / dkv; q, k, v, o, do, dq, dk, dv once: 48 us for all three).  16 pairs of 4096 rows on 1568 .. 3136 keys, hd 128: 140 us (105 GFLOP at full length),
-// dq 180, dkv 270-295: products, exponentials and LDS reads of a tile take about the same time and overlap by half.
+// What bounds it, measured (bf16): 256 captions of 5 .. 77 tokens on 197 keys, 8 heads of 64 (mean 41 rows a pair): latency of short blocks, 32 / 54 / 60 us
+// (fwd / dq / dkv; q, k, v, o, do, dq, dk, dv once: 48 us for all three).  16 pairs of 4096 rows on 1568 .. 3136 keys, hd 128: 140-150 us (105 GFLOP at full length),
+// dq 315, dkv 270-295: products, exponentials and LDS reads of a tile take about the same time and overlap by half.
 // 24 pairs of 2047 rows on 6272 keys, hd 64: 102 + 9 us = 700 TFLOP/s, the exponentials alone take 103 us at the full vector rate.  64 sequences of one token, 4 kv heads,
 // up to 3136 keys: 27 + 7 us, 129 MB = 4.8 TB/s.  fp32: 64-cycle instructions in a chain, 16 sequences of up to 77 on 257, 12 heads of 80: 40 / 50 / 44 us.
 //
@@ -35,7 +36,7 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 struct XP {
   const void *q, *k, *v, *o, *dout;
   void *out, *dq, *dk, *dv;
-  float *lse, *delta, *part_o, *part_ml;
+  float *lse, *delta, *part_o, *part_ml, *part_d;
   const int *cu_q, *cu_kv, *kv_len;
   const uint8_t* key_mask;
   long ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;
@@ -606,10 +607,26 @@ __global__ __launch_bounds__(256) void xattn_sum_kernel(const float* part, T* ou
   }
 }
 
+// a value the compiler knows nothing about: what follows from it is computed again where it is used
+__device__ __forceinline__ int opaque(int v) {
+#ifndef DH_HOST_EMU
+  asm volatile("" : "+v"(v));
+#endif
+  return v;
+}
+
 // ------------------------------------------------------------------------------------------ backward: dq (and D)
-template <typename T, int HDP, int RW, int BN, bool SPLIT>
+// D = sum(do o) = sum p dp.  Where the softmax has most of its weight on a few keys dp - D cancels, and a D formed from o as it was rounded to bf16 is off by
+// more than dS's own rounding: dq and dk by 7.8e-3 of their norm instead of 2.3e-3 (hd 64, 40 rows, q and k of deviation 3, 33 keys or more; two keys left
+// of 700: 3.9e-3 instead of 2.0e-3).  So bf16 sums p dp itself over all keys in front of the pass that forms dS, S and dP formed twice: 36 -> 54 us for
+// the captions, 191 -> 315 for the 16 pairs of 4096 rows.  fp32, whose o is as exact as p dp is, reads o.
+// WHOLE: a block meets all keys, twice.  RANGE: the keys in ranges, each range's dq a partial sum; in front of it (bf16) RANGE_D, whose blocks leave their
+// range's share of D.
+enum Part { WHOLE, RANGE, RANGE_D };
+template <typename T, int HDP, int RW, int BN, Part PART>
 __global__ __launch_bounds__(64 * RW, (waves_dq<T, HDP, RW>())) void xattn_dq_kernel(XP p) {
   constexpr int EPC = Op<T>::EPC, KS = HDP / (2 * EPC), DB = HDP / 32, NB = BN / 32, BM = 32 * RW, NT = 64 * RW;
+  constexpr bool SPLIT = PART != WHOLE, OWN_D = sizeof(T) == 2 && PART != RANGE;      // OWN_D: this block sums p dp over its keys
   DH_DYN_LDS_A16(unsigned char, smem);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
   if ((int)blockIdx.x >= p.main_blocks) {
@@ -634,55 +651,63 @@ __global__ __launch_bounds__(64 * RW, (waves_dq<T, HDP, RW>())) void xattn_dq_ke
     typename Op<T>::Frag qf[KS], df[KS];
     load_row<T, HDP>(qf, (const T*)p.q + (has ? m_offset(p, s, w.g, m, p.ldq) : 0), has, p.hd, h);
     load_row<T, HDP>(df, (const T*)p.dout + (has ? m_offset(p, s, w.g, m, p.lddo) : 0), has, p.hd, h);
+    Tiles<T, HDP, BN, NT> kt_(p, s, w.g, smem);
+    const T *Ks, *Vs;
+    const float* bias;
+    bool masked;
+    auto p_dp = [&](int b, f32x16_t& sc, f32x16_t& dp, int lane) {     // p and dp of 32 keys
+      sc = mma_row<T, HDP>(Ks, b * 32, qf, lane);
+      dp = mma_row<T, HDP>(Vs, b * 32, df, lane);
+      if (masked) mask_keys(sc, bias + b * 32, lane >> 5);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[i] = exp2_fast(fmaf(sc[i], c, -lse2));
+    };
     float D = 0.f;
-    {
+    if constexpr (OWN_D) {
+      const int tid = opaque(threadIdx.x), lane = tid & 63;    // (places in the tiles that the two passes do not share: shared, they spill in the second)
+      kt_.begin(lo, hi, tid);
+      for (int kt = lo; kt < hi; ++kt) {
+        masked = kt_.next(kt, hi, tid, Ks, Vs, bias);
+        if (wave_live) {
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            f32x16_t sc, dp;
+            p_dp(b, sc, dp, lane);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) D = fmaf(sc[i], dp[i], D);
+          }
+        }
+        __syncthreads();
+      }
+      D += other_half(D);
+    } else if constexpr (sizeof(T) == 2) {
+      if (live)
+        for (int i = 0; i < p.nsplit; ++i) D += p.part_d[(long)i * p.heads * p.rows_q + stat];
+    } else {
       typename Op<T>::Frag of[KS];
       load_row<T, HDP>(of, (const T*)p.o + (has ? m_offset(p, s, w.g, m, p.ldo) : 0), has, p.hd, h);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) D += Op<T>::dot(df[ks], of[ks]);
+      D += other_half(D);
     }
-    D += other_half(D);
+    if constexpr (PART == RANGE_D) {
+      if (live && h == 0) p.part_d[(long)w.split * p.heads * p.rows_q + stat] = D;
+      continue;
+    }
     if (live && h == 0 && (!SPLIT || w.split == 0)) p.delta[stat] = D;
     f32x16_t dq[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) dq[d][i] = 0.f;
-    Tiles<T, HDP, BN, NT> kt_(p, s, w.g, smem);
-    kt_.begin(lo, hi, tid);
+    if (!OWN_D || hi - lo > 1) kt_.begin(lo, hi, tid);         // (an only tile is still in LDS)
     for (int kt = lo; kt < hi; ++kt) {
-      const T *Ks, *Vs;
-      const float* bias;
-      const bool masked = kt_.next(kt, hi, tid, Ks, Vs, bias);
-      const bool busy = wave_live;
-      auto p_dp = [&](int b, f32x16_t& sc, f32x16_t& dp) {     // p and dp of 32 keys
-        sc = mma_row<T, HDP>(Ks, b * 32, qf, lane);
-        dp = mma_row<T, HDP>(Vs, b * 32, df, lane);
-        if (masked) mask_keys(sc, bias + b * 32, h);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sc[i] = exp2_fast(fmaf(sc[i], c, -lse2));
-      };
-      if (sizeof(T) == 2 && nt == 1) {
-        // all keys are here: D = sum p dp, which is sum(do o) before o was rounded.  With a few keys dp - D cancels, and the rounding of o
-        // alone would double the error of dq and dk (two keys: 3.6e-3 instead of 2.4e-3 of their norm); over many keys |o| is small against |v|.
-        D = 0.f;
-        if (busy) {
-#pragma unroll
-          for (int b = 0; b < NB; ++b) {
-            f32x16_t sc, dp;
-            p_dp(b, sc, dp);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) D = fmaf(sc[i], dp[i], D);
-          }
-        }
-        D += other_half(D);
-        if (live && h == 0 && (!SPLIT || w.split == 0)) p.delta[stat] = D;
-      }
-      if (busy) {
+      masked = kt_.next(kt, hi, tid, Ks, Vs, bias);
+      if (wave_live) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
           f32x16_t sc, dp;
-          p_dp(b, sc, dp);
+          p_dp(b, sc, dp, lane);
 #pragma unroll
           for (int i = 0; i < 16; ++i) sc[i] *= dp[i] - D;
           const typename Op<T>::PF pf = Op<T>::pack(sc);
@@ -699,14 +724,6 @@ __global__ __launch_bounds__(64 * RW, (waves_dq<T, HDP, RW>())) void xattn_dq_ke
       rows_out<T, HDP>(smem, dq, p.scale, p.hd, tid, [&](int r) -> T* { return t * BM + r < M ? (T*)p.dq + m_offset(p, s, w.g, t * BM + r, p.lddq) : nullptr; });
     }
   }
-}
-
-// a value the compiler knows nothing about: what follows from it is computed again where it is used
-__device__ __forceinline__ int opaque(int v) {
-#ifndef DH_HOST_EMU
-  asm volatile("" : "+v"(v));
-#endif
-  return v;
 }
 
 // ------------------------------------------------------------------------------------------ backward: dk, dv
@@ -967,7 +984,10 @@ int fwd_shape(XP& p, int64_t grid, hipStream_t st) {
 template <typename T, int HDP, int RW, int BN>
 int dq_shape(XP& p, int64_t grid, hipStream_t st) {
   const size_t lds = lds_bytes<T, HDP, RW>(BN, 1, p.nsplit > 1);
-  return p.nsplit > 1 ? launch(xattn_dq_kernel<T, HDP, RW, BN, true>, p, grid, 64 * RW, lds, st) : launch(xattn_dq_kernel<T, HDP, RW, BN, false>, p, grid, 64 * RW, lds, st);
+  if (p.nsplit == 1) return launch(xattn_dq_kernel<T, HDP, RW, BN, WHOLE>, p, grid, 64 * RW, lds, st);
+  if constexpr (sizeof(T) == 2)
+    if (int e = launch(xattn_dq_kernel<T, HDP, RW, BN, RANGE_D>, p, p.main_blocks, 64 * RW, lds, st)) return e;
+  return launch(xattn_dq_kernel<T, HDP, RW, BN, RANGE>, p, grid, 64 * RW, lds, st);
 }
 template <typename T, int HDP, int RW>
 int dkv_shape(XP& p, int64_t grid, hipStream_t st) {
@@ -1021,11 +1041,17 @@ int join_ranges(const XP& p, hipStream_t st) {
   DH_CHECK_LAUNCH();
   return DH_OK;
 }
+// the ranges' shares of D
+int64_t part_d_floats(const dh_xattn_args* a) {
+  const int64_t ns = plan_dq(a).nsplit;
+  return a->dtype == DH_BF16 && ns > 1 ? round4(ns * a->heads * a->rows_q) : 0;
+}
 template <typename T>
 int bwd(const dh_xattn_args* a, hipStream_t st) {
   XP p = params(a);
   p.delta = (float*)a->ws;
-  p.part_o = p.delta + round4((int64_t)a->heads * a->rows_q);
+  p.part_d = p.delta + round4((int64_t)a->heads * a->rows_q);
+  p.part_o = p.part_d + part_d_floats(a);
   int64_t grid;
   if (a->rows_q > 0) {
     const Plan pl = plan_dq(a);
@@ -1051,10 +1077,10 @@ int64_t fwd_bytes(const dh_xattn_args* a) {
   const int64_t ns = plan_fwd(a).nsplit;
   return ns > 1 ? ns * a->heads * a->rows_q * (a->hd + 2) * 4 : 0;
 }
-int64_t bwd_bytes(const dh_xattn_args* a) {       // D, and the larger of the partial dq and the partial dk, dv
+int64_t bwd_bytes(const dh_xattn_args* a) {       // D, its ranges' shares, and the larger of the partial dq and the partial dk, dv
   const int64_t sq = plan_dq(a).nsplit, sk = plan_dkv(a).nsplit;
   const int64_t q = sq > 1 ? sq * a->rows_q * a->heads * a->hd : 0, kv = sk > 1 ? 2 * sk * a->rows_kv * a->kv_heads * a->hd : 0;
-  return (round4((int64_t)a->heads * a->rows_q) + (q > kv ? q : kv)) * 4;
+  return (round4((int64_t)a->heads * a->rows_q) + part_d_floats(a) + (q > kv ? q : kv)) * 4;
 }
 
 }  // namespace

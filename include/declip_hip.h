@@ -203,7 +203,7 @@ int dh_attn_pooled_bwd(int dtype, const void* q, const void* kv, const void* dou
  *   max_q / max_kv: longest query / key row count of a sequence as far as the caller knows it (0: unknown), used to lay out the grid only --
  *   longer sequences are computed whole.  Table entries are clamped to the row counts, so no table makes a kernel leave its buffers.
  *   scale > 0.  bf16: P and dS are rounded to bf16 as MFMA operands; statistics, sums and accumulators fp32.  No atomics: the same bits on every run.
- * fwd reads q k v, writes out lse; bwd reads q k v out dout lse, writes dq dk dv.  ws: dh_xattn_ws_bytes(args, backward) bytes of scratch, 16-byte
+ * fwd reads q k v, writes out lse; bwd reads q k v dout lse (fp32: out too; bf16 forms sum(do out) from unrounded values), writes dq dk dv.  ws: dh_xattn_ws_bytes(args, backward) bytes of scratch, 16-byte
  * aligned, not shared with anything that may run at the same time. */
 typedef struct {
   int dtype, batch, heads, kv_heads, hd;
