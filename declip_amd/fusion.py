@@ -85,7 +85,8 @@ class JoinNormFn(torch.autograd.Function):
     @staticmethod
     def _named(params):
         post_w, post_b, gate, scale, pre_w, pre_b = params
-        return dict(post=None if post_w is None else (post_w, post_b), gate=gate, scale=scale, pre=None if pre_w is None else (pre_w, pre_b))
+        pair = lambda w, b: None if w is None and b is None else (w, b)  # noqa: E731 -- (a bias alone goes on, and is refused)
+        return dict(post=pair(post_w, post_b), gate=gate, scale=scale, pre=pair(pre_w, pre_b))
 
     @staticmethod
     @once_differentiable
