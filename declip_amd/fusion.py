@@ -15,6 +15,15 @@ from torch.autograd.function import once_differentiable
 
 from . import ops
 
+TABLES = ("cu_q", "cu_kv", "kv_len", "key_mask")
+
+
+def _number(v):
+    """a plain number, also of a tensor of one element: read once, in the forward, so that the backward goes by the same"""
+    if torch.is_tensor(v):
+        return v.detach().item()
+    return v
+
 
 def _rows16(t):
     """contiguous columns, 16-byte aligned rows less than 2^22 elements apart: what the kernels read; anything else is copied"""
@@ -47,6 +56,7 @@ class CrossAttnFn(torch.autograd.Function):
 
 def cross_attention(q, k, v, heads, *, need_lse=False, **geometry):
     """ops.xattn_fwd with its gradient: out [rows_q, heads*hd] (need_lse: (out, lse); lse carries no gradient)."""
+    geometry = {n: t if n in TABLES else _number(t) for n, t in geometry.items()}
     out, lse = CrossAttnFn.apply(q, k, v, heads, geometry)
     return (out, lse) if need_lse else out
 
@@ -68,6 +78,7 @@ class RopeAxesFn(torch.autograd.Function):
 
 def rope_axes(x, pos, heads, sections, theta=10000.0, *, joint=False, interleaved=False):
     """ops.rope_axes with its gradient (the rotation back); pos carries none."""
+    theta = tuple(_number(t) for t in theta) if isinstance(theta, (tuple, list)) else _number(theta)
     return RopeAxesFn.apply(x, pos, heads, tuple(sections), dict(theta=theta, joint=joint, interleaved=interleaved))
 
 
@@ -101,5 +112,6 @@ class JoinNormFn(torch.autograd.Function):
 
 def join_norm(x, y, *, post=None, gate=None, scale=None, pre=None, alpha=1.0, eps=1e-5, rms=False, gate_tanh=False):
     """ops.join_norm_fwd with its gradient: (x_out, n), n = None without `pre`."""
+    alpha, eps = _number(alpha), _number(eps)
     post, pre = post or (None, None), pre or (None, None)
     return JoinNormFn.apply(x, y, *post, gate, scale, *pre, dict(alpha=alpha, eps=eps, rms=rms, gate_tanh=gate_tanh))

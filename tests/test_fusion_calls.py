@@ -19,3 +19,26 @@ def test_a_bias_without_its_weight_is_refused(which):
         with pytest.raises(DeclipHipError, match="weight"):
             fusion.join_norm(x, x, **{which: (None, b)})
         assert fusion.join_norm(x, x, **{which: (None, None)})[1] is None
+
+
+def test_the_backward_takes_the_numbers_the_forward_took():
+    """alpha, theta and the like may come as tensors or lists that a schedule writes to before the backward runs"""
+    from declip_amd import fusion
+    with emulated_gpu():
+        x, y = rnd(4, 64).requires_grad_(True), rnd(4, 64, seed=1).requires_grad_(True)
+        alpha = torch.tensor(2.0)
+        out, _ = fusion.join_norm(x, y, alpha=alpha)
+        alpha.fill_(5.0)
+        dx, dy = torch.autograd.grad(out, [x, y], torch.ones_like(out))
+        assert torch.equal(dx, torch.full_like(x, 2.0)) and torch.equal(dy, torch.ones_like(y))
+        pos, theta, sections = torch.arange(4, dtype=torch.int32)[:, None].contiguous(), [100.0], [16]
+        out = fusion.rope_axes(x, pos, 2, sections, theta)
+        theta[0], sections[0] = 1e6, 8
+        back, = torch.autograd.grad(out, [x], out.detach())
+        assert float((back - x).abs().max()) < 1e-5          # rotated there and back
+        scale, most = torch.tensor(0.5), torch.tensor(4)
+        a, = torch.autograd.grad(fusion.cross_attention(x, y, y, 2, batch=1, scale=0.5).sum(), [x])
+        out = fusion.cross_attention(x, y, y, 2, batch=1, scale=scale, max_q=most)
+        scale.fill_(0.1)
+        b, = torch.autograd.grad(out.sum(), [x])
+        assert torch.equal(a, b)
