@@ -14,13 +14,16 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import ops
+from .lib import DeclipHipError
 
 TABLES = ("cu_q", "cu_kv", "kv_len", "key_mask")
 
 
-def _number(v):
-    """a plain number, also of a tensor of one element: read once, in the forward, so that the backward goes by the same"""
+def _number(name, v):
+    """a plain number, also of a tensor of one element: read once, in the forward, so that the backward goes by the same; one that asks for a gradient would get none"""
     if torch.is_tensor(v):
+        if v.requires_grad and torch.is_grad_enabled():
+            raise DeclipHipError("bad argument: %s carries no gradient (detach it, or multiply outside)" % name)
         return v.detach().item()
     return v
 
@@ -55,8 +58,8 @@ class CrossAttnFn(torch.autograd.Function):
 
 
 def cross_attention(q, k, v, heads, *, need_lse=False, **geometry):
-    """ops.xattn_fwd with its gradient: out [rows_q, heads*hd] (need_lse: (out, lse); lse carries no gradient)."""
-    geometry = {n: t if n in TABLES else _number(t) for n, t in geometry.items()}
+    """ops.xattn_fwd with its gradient: out [rows_q, heads*hd] (need_lse: (out, lse); lse and scale carry no gradient)."""
+    geometry = {n: t if n in TABLES else _number(n, t) for n, t in geometry.items()}
     out, lse = CrossAttnFn.apply(q, k, v, heads, geometry)
     return (out, lse) if need_lse else out
 
@@ -77,8 +80,8 @@ class RopeAxesFn(torch.autograd.Function):
 
 
 def rope_axes(x, pos, heads, sections, theta=10000.0, *, joint=False, interleaved=False):
-    """ops.rope_axes with its gradient (the rotation back); pos carries none."""
-    theta = tuple(_number(t) for t in theta) if isinstance(theta, (tuple, list)) else _number(theta)
+    """ops.rope_axes with its gradient (the rotation back); pos and theta carry none."""
+    theta = tuple(_number("theta", t) for t in theta) if isinstance(theta, (tuple, list)) else _number("theta", theta)
     return RopeAxesFn.apply(x, pos, heads, tuple(sections), dict(theta=theta, joint=joint, interleaved=interleaved))
 
 
@@ -111,7 +114,7 @@ class JoinNormFn(torch.autograd.Function):
 
 
 def join_norm(x, y, *, post=None, gate=None, scale=None, pre=None, alpha=1.0, eps=1e-5, rms=False, gate_tanh=False):
-    """ops.join_norm_fwd with its gradient: (x_out, n), n = None without `pre`."""
-    alpha, eps = _number(alpha), _number(eps)
+    """ops.join_norm_fwd with its gradient: (x_out, n), n = None without `pre`; alpha and eps carry none."""
+    alpha, eps = _number("alpha", alpha), _number("eps", eps)
     post, pre = post or (None, None), pre or (None, None)
     return JoinNormFn.apply(x, y, *post, gate, scale, *pre, dict(alpha=alpha, eps=eps, rms=rms, gate_tanh=gate_tanh))

@@ -42,3 +42,19 @@ def test_the_backward_takes_the_numbers_the_forward_took():
         scale.fill_(0.1)
         b, = torch.autograd.grad(out.sum(), [x])
         assert torch.equal(a, b)
+
+
+def test_a_trainable_number_is_refused():
+    """a learned scale, alpha or base: these operators have no gradient for it, and would leave it where it is without a word"""
+    from declip_amd import fusion
+    from declip_amd.lib import DeclipHipError
+    with emulated_gpu():
+        x, pos, t = rnd(4, 64), torch.arange(4, dtype=torch.int32)[:, None].contiguous(), torch.tensor(2.0, requires_grad=True)
+        for call, name in ((lambda v: fusion.cross_attention(x, x, x, 2, batch=1, scale=v), "scale"), (lambda v: fusion.join_norm(x, x, alpha=v), "alpha"),
+                           (lambda v: fusion.join_norm(x, x, eps=v), "eps"), (lambda v: fusion.rope_axes(x, pos, 2, (4,), theta=v), "theta"),
+                           (lambda v: fusion.rope_axes(x, pos, 2, (4,), theta=[v]), "theta")):
+            with pytest.raises(DeclipHipError, match=name):
+                call(t)
+            call(t.detach())
+            with torch.no_grad():
+                call(t)
