@@ -251,13 +251,26 @@ def self_launch(n):
     return rc
 
 
+def _end_with_parent():
+    """A second attempt (DH_BENCH_PARENT: the rank's first process) ends when that process does, however that ends: launchers terminate or kill the
+    one process they started, and an attempt left behind would hold the card and the rendezvous port."""
+    parent = os.environ.pop("DH_BENCH_PARENT", None)
+    if parent is None:
+        return
+    import ctypes
+    import signal
+    PR_SET_PDEATHSIG = 1
+    ctypes.CDLL(None).prctl(PR_SET_PDEATHSIG, int(signal.SIGKILL), 0, 0, 0)
+    if os.getppid() != int(parent):              # it ended before the line above
+        os._exit(1)
+
+
 def _arm_watchdog(seconds, what):
     """Last line of defence for the DEFAULT multi-GPU configuration (captured step with RCCL collectives in the graph), which has
     never run on more than one rank: if `what` makes no progress for `seconds`, this rank re-executes itself with --graph 0.  A hang
     inside a collective stops every rank, so every rank's watchdog fires and the re-executed ranks meet again in a fresh rendezvous
     (torchrun: the agent's store with the next attempt prefix; self-launched: the next port).  The new attempt is a child process -- a
-    program that has initialised the GPU must not exec -- whose exit code becomes this rank's; this process does nothing more but wait
-    for it (its queues, hung or not, go when it ends).  The line then carries `graph_fallback`.  Returns the timer (cancel())."""
+    program that has initialised the GPU must not exec -- whose exit code becomes this rank's and which ends with it (`_end_with_parent`).  The line then carries `graph_fallback`.  Returns the timer (cancel())."""
     import subprocess
     import threading
 
@@ -268,7 +281,7 @@ def _arm_watchdog(seconds, what):
         msg = msg or "watchdog: %s made no progress in %d s; rank re-executed with --graph 0" % (what, int(seconds))
         sys.stderr.write("bench.py: " + msg + "\n")
         sys.stderr.flush()
-        env = dict(os.environ, DH_BENCH_GRAPH_FALLBACK=msg)
+        env = dict(os.environ, DH_BENCH_GRAPH_FALLBACK=msg, DH_BENCH_PARENT=str(os.getpid()))
         if env.get("TORCHELASTIC_USE_AGENT_STORE") == "True":
             env["TORCHELASTIC_RESTART_COUNT"] = str(int(env.get("TORCHELASTIC_RESTART_COUNT", "0")) + 1)     # fresh key prefix in the agent's store
         elif env.get("MASTER_PORT", "").isdigit():
@@ -337,6 +350,7 @@ def dry_run_launch(args):
 
 
 def main():
+    _end_with_parent()
     ap = argparse.ArgumentParser()
     ap.add_argument("--gpus", type=int, default=1)
     ap.add_argument("--steps", type=int, default=10)
