@@ -265,53 +265,87 @@ def _end_with_parent():
         os._exit(1)
 
 
-def _arm_watchdog(seconds, what):
+class _Watchdog:
     """Last line of defence for the DEFAULT multi-GPU configuration (captured step with RCCL collectives in the graph), which has
-    never run on more than one rank: if `what` makes no progress for `seconds`, this rank re-executes itself with --graph 0.  A hang
-    inside a collective stops every rank, so every rank's watchdog fires and the re-executed ranks meet again in a fresh rendezvous
-    (torchrun: the agent's store with the next attempt prefix; self-launched: the next port).  The new attempt is a child process -- a
-    program that has initialised the GPU must not exec -- whose exit code becomes this rank's and which ends with it (`_end_with_parent`).  The line then carries `graph_fallback`.  Returns the timer (cancel())."""
-    import subprocess
-    import threading
+    never run on more than one rank: if `what` makes no progress for `seconds`, this rank starts over with --graph 0.  A hang
+    inside a collective stops every rank, so every rank's watchdog fires and the second attempts meet again in a fresh rendezvous
+    (torchrun: the agent's store with the next attempt prefix; self-launched: the next port).  The second attempt is a child process -- a
+    program that has initialised the GPU must not exec -- whose exit code becomes this rank's and which ends with it (`_end_with_parent`).
+    This process keeps its context, and a kernel that hangs may keep part of the card busy, until then: the line's `graph_fallback` says so.
+    Once the second attempt is under way it alone speaks for the rank: the thread that `what` runs on comes to rest at the next `check`, or when
+    `what` returns or raises (`guard`)."""
 
-    fired = threading.Event()
+    def __init__(self, seconds, what):
+        import threading
+        self._lock, self._over, self._started, self._waiter = threading.Lock(), False, False, None
+        self._what, self._seconds = what, seconds
+        self._timer = threading.Timer(seconds, self._fire)
+        self._timer.daemon = True
+        self._timer.start()
 
-    def fire(msg=None):
-        fired.set()
-        msg = msg or "watchdog: %s made no progress in %d s; rank re-executed with --graph 0" % (what, int(seconds))
-        sys.stderr.write("bench.py: " + msg + "\n")
-        sys.stderr.flush()
-        env = dict(os.environ, DH_BENCH_GRAPH_FALLBACK=msg, DH_BENCH_PARENT=str(os.getpid()))
-        if env.get("TORCHELASTIC_USE_AGENT_STORE") == "True":
-            env["TORCHELASTIC_RESTART_COUNT"] = str(int(env.get("TORCHELASTIC_RESTART_COUNT", "0")) + 1)     # fresh key prefix in the agent's store
-        elif env.get("MASTER_PORT", "").isdigit():
-            env["MASTER_PORT"] = str(int(env["MASTER_PORT"]) + 1)                                              # rank 0 hosts the store itself: next port
-        argv, skip = [], False
-        for a in sys.argv[1:]:
-            if skip:
-                skip = False
-                continue
-            if a == "--graph":
-                skip = True
-                continue
-            if a.startswith("--graph="):
-                continue
-            argv.append(a)
-        # (the old rendezvous' sockets stay with this process: the new one uses another port)
-        code = subprocess.call([sys.executable, os.path.abspath(__file__)] + argv + ["--graph", "0"], env=env, stdout=_JSON_FD)      # None: stdout as it is
-        os._exit(code if code >= 0 else 128 - code)
-    t = threading.Timer(seconds, fire)
-    t.daemon = True
-    stop = t.cancel
+    def _fire(self):
+        import threading
+        with self._lock:
+            if self._over:                        # cancelled in the moment that it went off
+                return
+            self._started, self._waiter = True, threading.current_thread()
+        self._second_attempt("watchdog: %s made no progress in %d s; rank started over with --graph 0 beside the hung process" % (self._what, int(self._seconds)))
 
-    def cancel():
-        stop()
-        if fired.is_set():
-            t.join()          # (the step came back after all, too late: the new attempt speaks for this rank, and ends it)
-    t.cancel = cancel
-    t.reexec = fire           # the same way out for a captured step that RAISES (GraphedStep: invalidated capture / failed first launch)
-    t.start()
-    return t
+    def check(self):
+        """does not return once the second attempt has been started"""
+        with self._lock:
+            started = self._started
+        if started:
+            self._waiter.join()                   # (ends the process with the attempt's exit code)
+
+    def cancel(self):
+        with self._lock:
+            self._over = True
+        self._timer.cancel()
+        self.check()
+
+    def start_over(self, why):
+        """the same way out for a captured step that RAISES (GraphedStep: invalidated capture / failed first launch); does not return"""
+        self.cancel()
+        self._second_attempt("captured step unusable (%s); rank started over with --graph 0 beside the first process" % why)
+
+    def guard(self, run):
+        """run(), whose return or exception counts only if there is no second attempt; disarmed behind it"""
+        try:
+            run()
+        finally:
+            self.cancel()
+
+    def _second_attempt(self, msg):
+        import subprocess
+        code = 1
+        try:
+            sys.stderr.write("bench.py: " + msg + "\n")
+            sys.stderr.flush()
+            env = dict(os.environ, DH_BENCH_GRAPH_FALLBACK=msg, DH_BENCH_PARENT=str(os.getpid()))
+            if env.get("TORCHELASTIC_USE_AGENT_STORE") == "True":
+                env["TORCHELASTIC_RESTART_COUNT"] = str(int(env.get("TORCHELASTIC_RESTART_COUNT", "0")) + 1)     # fresh key prefix in the agent's store
+            elif env.get("MASTER_PORT", "").isdigit():
+                env["MASTER_PORT"] = str(int(env["MASTER_PORT"]) + 1)                                              # rank 0 hosts the store itself: next port
+            argv, skip = [], False
+            for a in sys.argv[1:]:
+                if skip:
+                    skip = False
+                    continue
+                if a == "--graph":
+                    skip = True
+                    continue
+                if a.startswith("--graph="):
+                    continue
+                argv.append(a)
+            # (the old rendezvous' sockets stay with this process: the new one uses another port)
+            code = subprocess.call([sys.executable, os.path.abspath(__file__)] + argv + ["--graph", "0"], env=env, stdout=_JSON_FD)      # None: stdout as it is
+        finally:
+            os._exit(code if code >= 0 else 128 - code)
+
+
+def _arm_watchdog(seconds, what):
+    return _Watchdog(seconds, what)
 
 
 def dry_run_launch(args):
@@ -461,13 +495,13 @@ def main():
     # Round 5: a multi-GPU rank runs the captured step by DEFAULT too (RCCL collectives captured with it; the one-rank capture is tested in
     # tests/test_gpu_dist.py, DH_DIST_FORCE=1 runs it here) -- with two safety nets, because W > 1 has never executed anywhere: a capture
     # that raises falls back to the eager step on EVERY rank (GraphedStep(fallback=True, agree=...)), and a warm-up that makes no progress
-    # (a collective hanging inside a replay) re-executes the rank with --graph 0 (`_arm_watchdog`); either way the line says so in
+    # (a collective hanging inside a replay) starts the rank over with --graph 0 (`_Watchdog`); either way the line says so in
     # `graph_fallback`.  Never over a gloo group (host-side collectives).
     graph_default = "1" if args.model in ("clip", "clip_r50", "filip", "declip", "defilip", "slip") else "0"
     use_graph = (args.graph if args.graph is not None else os.environ.get("DH_STEP_GRAPH", graph_default)) == "1"
     if world > 1 and torch.distributed.get_backend() != "nccl":
         use_graph = False
-    graph_fallback = os.environ.get("DH_BENCH_GRAPH_FALLBACK")        # set by a watchdog re-execution of this rank
+    graph_fallback = os.environ.get("DH_BENCH_GRAPH_FALLBACK")        # set for a second attempt of this rank
     # sanity of a multi-GPU launch before anything is timed: every rank of the launch is in the communicator (a SUM all-reduce of
     # ones over RCCL must count `world` ranks) and sits on its own device
     rccl_ranks = 1
@@ -540,6 +574,8 @@ def main():
     watchdog = _arm_watchdog(float(os.environ.get("DH_GRAPH_WATCHDOG_S", "240")), "the warm-up of the captured multi-GPU step") if (dist_on and use_graph) else None
 
     def step():
+        if watchdog is not None:
+            watchdog.check()                     # (a step that came back too late)
         if pipeline is not None:
             nxt = pipeline.next()                # the caller's stream waits for the copy stream's event: no host synchronisation
             if use_graph:
@@ -562,27 +598,31 @@ def main():
             p_.data.clamp_(3, 6)
         return loss
 
-    try:
+    def warm_up():
         for _ in range(args.warmup):
             step()
         while use_graph and graphed.enabled and graphed.graph is None:
             step()             # fewer warm-up steps than the capture needs (2 eager + 1 captured): the capture must not land in the timed region
+        if watchdog is not None and graphed.enabled and graphed.graph is not None:
+            if os.environ.get("DH_BENCH_TEST_HANG") == "1" and not graph_fallback:      # test hook: a replay that never returns (tests/test_gpu_bench_fallback.py)
+                time.sleep(3600)
+            step()             # two replays, waited for, before the watchdog is disarmed: a collective that hangs in a replay hangs here
+            step()
+            torch.cuda.synchronize()
+
+    try:
+        if watchdog is None:
+            warm_up()
+        else:
+            watchdog.guard(warm_up)
     except RuntimeError as e:
         # a data-parallel rank whose captured step cannot be used and cannot be replaced by the eager step IN THIS PROCESS (GraphedStep:
         # the capture was invalidated, or the first launch failed after the peers entered theirs): the same way out as a hang --
         # this rank starts over with --graph 0; its peers, stuck in a collective without it, follow through their watchdogs
         if watchdog is None or "GraphedStep" not in str(e) or graph_fallback:
             raise
-        watchdog.cancel()
-        watchdog.reexec("captured step unusable (%s); rank re-executed with --graph 0" % str(e).splitlines()[0][:200])
-    if watchdog is not None:
-        if graphed.enabled and graphed.graph is not None:
-            if os.environ.get("DH_BENCH_TEST_HANG") == "1" and not graph_fallback:      # test hook: a replay that never returns (tests/test_gpu_bench_fallback.py)
-                time.sleep(3600)
-            step()             # two replays, waited for, before the watchdog is disarmed: a collective that hangs in a replay hangs here
-            step()
-            torch.cuda.synchronize()
-        watchdog.cancel()
+        watchdog.start_over(str(e).splitlines()[0][:200])
+    watchdog = None            # (disarmed: the timed steps look at nothing)
     if graphed.fallback_reason and not graph_fallback:
         graph_fallback = graphed.fallback_reason
     if use_graph and graph_key is not None:

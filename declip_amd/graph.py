@@ -175,7 +175,7 @@ class GraphedStep(object):
                     # the capture itself was INVALIDATED (an operation that is illegal under capture ran): torch.cuda.graph's exit raised
                     # from capture_end() before it restored the stream and told the allocator that the capture is over.  There is no
                     # eager step to fall back to in this process (measured: the next synchronisation aborts it) -- end the HIP-side
-                    # capture so that teardown is clean, and fail loudly; bench.py re-executes the rank with --graph 0.
+                    # capture so that teardown is clean, and fail loudly; bench.py starts the rank over with --graph 0.
                     self._abandon_capture(before)
                     self.enabled, self.fallback_reason = False, "capture invalidated (%s)" % err
                     raise RuntimeError("GraphedStep: the stream capture of the step was invalidated and cannot be recovered from in this "

@@ -78,3 +78,32 @@ def test_the_second_attempt_ends_with_its_rank(sig, ready):
             except OSError:
                 pass
         p.communicate()
+
+
+@pytest.mark.parametrize("late", ["pass", "raise ValueError('the step came to nothing')", "[w.check() for w in [W]]; print('went on')"])
+def test_a_step_that_comes_back_too_late_says_nothing_more(late):
+    """the step returns, raises or begins the next one while the second attempt runs: the attempt's line and exit code are the rank's"""
+    p = _rank("W = bench._arm_watchdog(0.1, 'a step')\ndef late():\n    time.sleep(1.0)\n    %s\nW.guard(late)\nprint('went on')" % late, 1)
+    out, err = p.communicate(timeout=120)
+    assert p.returncode == 0 and '"dry_run": true' in out and "went on" not in out and "ValueError" not in err, (out, err[-2000:])
+
+
+def test_a_step_in_time_disarms_the_watchdog():
+    p = _rank("W = bench._arm_watchdog(0.5, 'a step')\nW.guard(lambda: None)\nW._fire()\ntime.sleep(1.0)\nW.check()\nprint('went on')", 1)
+    out, err = p.communicate(timeout=120)
+    assert p.returncode == 0 and out.strip() == "went on" and "watchdog" not in err
+    p = _rank("W = bench._arm_watchdog(0.5, 'a step')\ndef bad():\n    raise ValueError('of its own')\nW.guard(bad)", 1)
+    out, err = p.communicate(timeout=120)
+    assert p.returncode == 1 and "of its own" in err and "watchdog" not in err
+
+
+def test_an_unusable_step_starts_over():
+    p = _rank("W = bench._arm_watchdog(60, 'a step')\nW.cancel()\nW.start_over('no capture')\nprint('went on')", 1)
+    out, err = p.communicate(timeout=120)
+    assert p.returncode == 0 and '"dry_run": true' in out and "went on" not in out and "captured step unusable (no capture)" in err
+
+
+def test_an_attempt_that_fails_fails_the_rank():
+    p = _rank("sys.argv += ['--gpus', '2']\nbench._arm_watchdog(0.1, 'a step')\ntime.sleep(600)", 1)     # (its world is 1)
+    out, err = p.communicate(timeout=120)
+    assert p.returncode == 3, err[-2000:]
