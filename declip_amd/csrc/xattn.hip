@@ -386,15 +386,15 @@ __device__ __forceinline__ void rows_out(unsigned char* smem, const f32x16_t* ac
 // of 77) dkv of 4 waves 97 / 79; fp32 hd 64 (16 sequences of 77) dkv 23 / 29, fwd of one wave 17.6 / 23.  RW: waves per block.
 template <typename T, int HDP, int RW, bool SPLIT> constexpr int waves_fwd() {
   constexpr int row = HDP * sizeof(T);
-  return SPLIT && RW == 4 && row <= 128 && sizeof(T) == 2 ? 3 : RW == 1 ? (row <= 64 ? 3 : sizeof(T) == 2 && row <= 128 ? 2 : 1) : RW == 2 ? (row <= 128 ? 3 : row <= 256 ? 2 : 1) : row <= 384 ? 2 : 1;
+  return SPLIT && RW == 4 && row <= 128 && sizeof(T) == 2 ? 3 : RW == 1 ? (row <= 64 ? 3 : sizeof(T) == 2 && row <= 128 ? 2 : 1) : row <= 384 ? 2 : 1;
 }
 template <typename T, int HDP, int RW> constexpr int waves_dq() {
   constexpr int row = HDP * sizeof(T);
-  return RW <= 2 && row <= 64 ? 3 : row <= 128 || RW == 8 ? 2 : RW == 1 ? 1 : RW == 2 ? (sizeof(T) == 2 ? 2 : 1) : row <= (sizeof(T) == 2 ? 192 : 256) ? 2 : 1;
+  return RW == 1 && row <= 64 ? 3 : row <= 128 || RW == 8 || (RW == 4 && row <= 256) ? 2 : 1;
 }
 template <typename T, int HDP, int RW> constexpr int waves_dkv() {
   constexpr int row = HDP * sizeof(T);
-  return RW <= 2 && row <= 64 ? 3 : row <= 128 || RW == 8 || (RW == 4 && row == 192) ? 2 : 1;
+  return RW == 1 && row <= 64 ? 3 : row <= 128 || RW == 8 || (RW == 4 && row == 192) ? 2 : 1;
 }
 
 // ------------------------------------------------------------------------------------------ forward
@@ -975,6 +975,7 @@ template <typename T, int HDP, int RW> constexpr size_t lds_bytes(int rows, int 
   const size_t out = split || sizeof(T) == 4 ? (size_t)RW * 32 * (HDP + 4) * 4 : (size_t)RW * 32 * (HDP + Op<T>::EPC) * sizeof(T);
   return tiles > out ? tiles : out;
 }
+int no_shape(int rw) { DH_FAIL(DH_ERR_ARG, "dh_xattn: no blocks of %d waves at this width", rw); }
 template <typename T, int HDP, int RW, int BN>
 int fwd_shape(XP& p, int64_t grid, hipStream_t st) {
   static_assert(lds_bytes<T, HDP, RW>(BN, 1, true) <= 160 * 1024, "LDS");
@@ -992,28 +993,41 @@ int dq_shape(XP& p, int64_t grid, hipStream_t st) {
 template <typename T, int HDP, int RW>
 int dkv_shape(XP& p, int64_t grid, hipStream_t st) {
   const size_t lds = lds_bytes<T, HDP, RW>(32, 2, p.nsplit > 1);
-  return p.nsplit > 1 ? launch(xattn_dkv_kernel<T, HDP, RW, true>, p, grid, 64 * RW, lds, st) : launch(xattn_dkv_kernel<T, HDP, RW, false>, p, grid, 64 * RW, lds, st);
+  if constexpr (RW != 2)                               // (two waves: up to 128 query rows, half of the least range)
+    if (p.nsplit > 1) return launch(xattn_dkv_kernel<T, HDP, RW, true>, p, grid, 64 * RW, lds, st);
+  if (p.nsplit > 1) return no_shape(RW);
+  return launch(xattn_dkv_kernel<T, HDP, RW, false>, p, grid, 64 * RW, lds, st);
 }
 
+// the block shapes that row_waves can ask for at this width: one and four waves; more than 64 columns of bf16 eight (dq instead of four); dk / dv of more
+// than 96 also two
+template <Kind K, typename T, int HDP> constexpr bool shape(int rw) {
+  const bool wide = sizeof(T) == 2 && HDP > 64;
+  return rw == 1 || (rw == 4 && !(wide && K == DQ)) || (rw == 8 && wide) || (rw == 2 && wide && K == DKV && HDP > 96);
+}
 template <typename T, int HDP>
 int fwd_hd(XP& p, int rw, int64_t grid, hipStream_t st) {
   constexpr int BN = sizeof(T) == 2 ? 64 : 32;
-  if constexpr (sizeof(T) == 2 && HDP > 64)
-    if (rw == 8) return fwd_shape<T, HDP, 8, BN>(p, grid, st);
-  return rw == 1 ? fwd_shape<T, HDP, 1, 32>(p, grid, st) : rw == 2 ? fwd_shape<T, HDP, 2, 32>(p, grid, st) : fwd_shape<T, HDP, 4, BN>(p, grid, st);
+  if (rw == 1) return fwd_shape<T, HDP, 1, 32>(p, grid, st);
+  if constexpr (shape<FWD, T, HDP>(4)) if (rw == 4) return fwd_shape<T, HDP, 4, BN>(p, grid, st);
+  if constexpr (shape<FWD, T, HDP>(8)) if (rw == 8) return fwd_shape<T, HDP, 8, BN>(p, grid, st);
+  return no_shape(rw);
 }
 template <typename T, int HDP>
 int dq_hd(XP& p, int rw, int64_t grid, hipStream_t st) {
   constexpr int BN = sizeof(T) == 2 ? 64 : 32;
-  if constexpr (sizeof(T) == 2 && HDP > 64)
-    if (rw == 8) return dq_shape<T, HDP, 8, BN>(p, grid, st);
-  return rw == 1 ? dq_shape<T, HDP, 1, 32>(p, grid, st) : rw == 2 ? dq_shape<T, HDP, 2, 32>(p, grid, st) : dq_shape<T, HDP, 4, BN>(p, grid, st);
+  if (rw == 1) return dq_shape<T, HDP, 1, 32>(p, grid, st);
+  if constexpr (shape<DQ, T, HDP>(4)) if (rw == 4) return dq_shape<T, HDP, 4, BN>(p, grid, st);
+  if constexpr (shape<DQ, T, HDP>(8)) if (rw == 8) return dq_shape<T, HDP, 8, BN>(p, grid, st);
+  return no_shape(rw);
 }
 template <typename T, int HDP>
 int dkv_hd(XP& p, int rw, int64_t grid, hipStream_t st) {
-  if constexpr (sizeof(T) == 2 && HDP > 64)
-    if (rw == 8) return dkv_shape<T, HDP, 8>(p, grid, st);
-  return rw == 1 ? dkv_shape<T, HDP, 1>(p, grid, st) : rw == 2 ? dkv_shape<T, HDP, 2>(p, grid, st) : dkv_shape<T, HDP, 4>(p, grid, st);
+  if (rw == 1) return dkv_shape<T, HDP, 1>(p, grid, st);
+  if constexpr (shape<DKV, T, HDP>(2)) if (rw == 2) return dkv_shape<T, HDP, 2>(p, grid, st);
+  if constexpr (shape<DKV, T, HDP>(4)) if (rw == 4) return dkv_shape<T, HDP, 4>(p, grid, st);
+  if constexpr (shape<DKV, T, HDP>(8)) if (rw == 8) return dkv_shape<T, HDP, 8>(p, grid, st);
+  return no_shape(rw);
 }
 
 template <typename T>
