@@ -793,8 +793,10 @@ __global__ __launch_bounds__(64 * RW, (waves_dkv<T, HDP, RW>())) void xattn_dkv_
     if (lo + 1 < hi_mt) fetch(lo + 1, tid);
     if (lo < hi_mt) __syncthreads();
     for (int mt = lo; mt < hi_mt; ++mt) {
-      // (a thread's places in the tiles are formed anew on every turn: kept, they are spilled, and a reload waits for all loads under way)
-      const int tid = opaque(threadIdx.x), lane = tid & 63, h = lane >> 5;
+      // A thread's places in the tiles are formed anew on every turn where kept ones are spilled, a reload waiting for all loads under way: more than 64
+      // columns (16 pairs of 4096 rows on 3136 keys, hd 128: 353 -> 312 us) and blocks of one wave (captions 59.7 -> 58.5 us; 197 rows on up to 77 keys 42.5 -> 44.4).
+      // Four waves of up to 64 columns have the registers: formed anew 30.2 / 36.4 us, kept 29.0 / 34.8 (16 x 512 on 512 / 32 x 197 on 577, 8 heads).
+      const int tid = HDP > 64 || RW == 1 ? opaque(threadIdx.x) : (int)threadIdx.x, lane = tid & 63, h = lane >> 5;
       if (mt + 1 < hi_mt) {
         store(mt + 1, tid);
         if (mt + 2 < hi_mt) fetch(mt + 2, tid);
