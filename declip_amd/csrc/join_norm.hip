@@ -278,6 +278,9 @@ template <typename T, int W, int NC, int V, bool ROWGATE>
 __global__ __launch_bounds__(NT, 2) void join_bwd_kernel(JP p) {
   DH_DYN_LDS_A16(float, sm);                      // three parameter vectors over the lanes' columns; behind the loop [G][d] for the groups' column sums
   constexpr int WIDE = 64 * W * NC * V;
+  // The next row on its way beside the current one, but for the shape of single elements (odd widths above 4096), whose 16 addresses and 16 columns of each of
+  // four operands and sums would spill up to 1513 registers: 2048 rows of 8191 1710 -> 323 us (fp32, one gate), 508 -> 296 (bf16); spills 130 and 113.
+  constexpr bool AHEAD = NC < 16;
   __shared__ float red[32];
   Lanes<W> ln;
   constexpr int G = Lanes<W>::G;
@@ -308,7 +311,7 @@ __global__ __launch_bounds__(NT, 2) void join_bwd_kernel(JP p) {
     if (p.post_w) { nst[0] = p.stats[row]; nst[1] = p.stats[p.rows + row]; }
     if (p.dn) { nst[2] = p.stats[2 * (long)p.rows + row]; nst[3] = p.stats[3 * (long)p.rows + row]; }
   };
-  if (first < last) fetch(first + ln.group);
+  if (AHEAD && first < last) fetch(first + ln.group);
   // read by every row from LDS: held in registers they would leave room for half of the waves
   for (int c = threadIdx.x; c < WIDE; c += NT) {
     float s = 0.f, w = 1.f, b = 0.f;               // (columns behind d add nothing to any sum)
@@ -332,6 +335,7 @@ __global__ __launch_bounds__(NT, 2) void join_bwd_kernel(JP p) {
   for (int row0 = first; row0 < last; row0 += G) {
     const int row = row0 + ln.group;
     const bool live = row < last;
+    if (!AHEAD) fetch(row);
     const float mu = nst[0], rs = nst[1], mu2 = nst[2], rs2 = nst[3], g = ROWGATE ? act(p, ng) : 1.f;
     float yh[NC][V], Gr[NC][V], xh[NC][V], wn[NC][V];
     float s1 = 0.f, s2 = 0.f;
@@ -355,7 +359,7 @@ __global__ __launch_bounds__(NT, 2) void join_bwd_kernel(JP p) {
         E[k][e] += dnv[e];
       }
     }
-    if (row0 + G < last) fetch(row + G);
+    if (AHEAD && row0 + G < last) fetch(row + G);
     if (p.dn) {
       ln.sum2(s1, s2, red);
       const float c1 = p.rms ? 0.f : -rs2 * s1 * inv_d, c2 = -rs2 * s2 * inv_d;
