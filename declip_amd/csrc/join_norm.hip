@@ -13,7 +13,9 @@
 // are fp32 and two-pass (mean first).  The column sums stay in registers over a block's rows, go to a partial row per block, and are
 // added in a fixed order by a second small kernel: no atomics, the same result on every run.
 // Measured, bf16: 25600 rows of 768, a gate vector per 50 rows: forward 33 us (157 MB: 4.8 TB/s), backward 55 + 8 us (236 MB: 4.2 TB/s); 8191 rows of 4096,
-// one gate: 51 us (268 MB: 5.3 TB/s), 97 + 8 us (403 MB: 4.2 TB/s).
+// one gate: 51 us (268 MB: 5.3 TB/s), 97 + 8 us (403 MB: 4.2 TB/s).  fp32: 61 and 110 + 10 us (314, 472 MB), 100 and 177 + 9 us (537, 805 MB).  What holds the backward below the
+// forward's rate: a block of 512 threads and 168 registers leaves room for no second one (two waves per SIMD, where 256 threads would allow three).
+// A gate vector per ROW is the slow case: a block and a partial row of 16 bytes per element for each, more than the call's own traffic (25600 x 768, bf16: 244, 702 + 352 us).
 #include "dh_common.h"
 #include <initializer_list>
 
@@ -551,7 +553,8 @@ int blocks_of(const dh_join_norm_args* a, int w, int most, int& per_group) {
   per_group = dh_cdiv(dh_cdiv(a->rows, n), g) * g;
   return dh_cdiv(a->rows, per_group);
 }
-// one block per compute unit: its column sums leave once (two rounds of blocks at 25600 x 768: 109 us against 55)
+// one block per compute unit, whose column sums leave once (two rounds of blocks at 25600 x 768: 109 us against 55) -- but with a gate vector per group of rows a block
+// per group at least (512 groups of 50 rows: two rounds)
 int bwd_blocks(const dh_join_norm_args* a, int w, int& per_group) { return blocks_of(a, w, j_cus(), per_group); }
 
 int check(const dh_join_norm_args* a, const char* who) {

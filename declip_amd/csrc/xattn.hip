@@ -18,11 +18,17 @@
 // it costs the results about as much as their own rounding (1.7e-3 of the norm each), and kept in two bf16 parts P and dS would double half of the
 // products.  Their sums (l, D) are formed before, in fp32.  fp32: v_mfma_f32_32x32x2_f32, nothing rounded.
 //
-// What bounds it, measured (bf16): 256 captions of 5 .. 77 tokens on 197 keys, 8 heads of 64 (mean 41 rows a pair): latency of short blocks, 32 / 54 / 60 us
-// (fwd / dq / dkv; q, k, v, o, do, dq, dk, dv once: 48 us for all three).  16 pairs of 4096 rows on 1568 .. 3136 keys, hd 128: 140-150 us (105 GFLOP at full length),
-// dq 315, dkv 270-295: products, exponentials and LDS reads of a tile take about the same time and overlap by half.
-// 24 pairs of 2047 rows on 6272 keys, hd 64: 102 + 9 us = 700 TFLOP/s, the exponentials alone take 103 us at the full vector rate.  64 sequences of one token, 4 kv heads,
-// up to 3136 keys: 27 + 7 us, 129 MB = 4.8 TB/s.  fp32: 64-cycle instructions in a chain, 16 sequences of up to 77 on 257, 12 heads of 80: 40 / 50 / 44 us.
+// What bounds it, measured (bf16):
+//   256 captions of 5 .. 77 tokens on 197 keys, 8 heads of 64: 32 / 54 / 60 us (fwd / dq / dkv), memory: 125 / 241 / 229 MB at 3.9 .. 4.5 TB/s.  Each tensor once would
+//   be 249 MB, 48 us for all three; k and v are read four times, q and do three.
+//   16 pairs of 4096 rows on 1568 .. 3136 keys, hd 128: 142 / 305 / 272 us = 740 / 860 / 770 TFLOP/s of matrix instructions at full lengths (dq's five
+//   products, two of them for D).  They hold the matrix units for 31 / 38 / 33 % of the cycles, vector instructions 42 / 39 / 27 %: one after
+//   the other in a wave, and two waves per SIMD cover part of it.  dkv has blocks for 208 of 256 compute units.
+//   24 pairs of 2047 rows on 6272 keys, hd 64: 104 + 9 us.  147 tiles of 32 rows and 64 keys per SIMD, each 512 cycles of matrix instructions and about 900 of vector
+//   ones (512 of them the 32 exponentials): 34 + 59 us at the 2.2 GHz it ran at, so the two hardly overlap.
+//   64 sequences of one token, 4 kv heads, up to 3136 keys: 27 + 7 us, 129 MB = 4.8 TB/s.
+//   fp32, 16 sequences of up to 77 on 257, 12 heads of 80: 40 / 50 / 44 us.  The 64-cycle matrix instructions of a block in a chain are 13 .. 19 of it (twice that where
+//   two blocks share a compute unit); half of the waves of 128-row blocks have no rows, a head of 80 is computed as 96, and the forward spills.
 //
 // Keys outside the sequence or masked: their rows are staged as ZEROS (whatever the memory holds, NaN included) and their scores are
 // -inf.  A row without a valid key: o = 0, lse = -inf, no gradient.  Rows that no sequence owns are written as zeros (lse -inf).
@@ -871,7 +877,10 @@ enum Kind { FWD, DQ, DKV };
 // on 197 keys fwd 31 / 39 / 42, dq 36 / 52 / 48, dkv 58 / 60 / 62; 197 rows on 5 .. 77 keys fwd 42 / 37 / 48, dq 58 / 65 / 72; 128 pairs of 512 on 512 fwd
 // 26 / 23 / 18, dkv 39 / 32 / 29; 24 pairs of 2047 on 6272 fwd 226 / 198 / 147.
 // More than 64 columns: eight waves (half of the staging registers each, two waves per SIMD) once they are filled: 16 pairs of 4096 rows on 3136 keys fwd
-// 164 (four: 170), dq 191 (319), dkv 382 (612; both before the padding and the spill-free loop below).  fp32 is bound by its matrix instructions: four.
+// 164 (four: 170), dq 191 (319), dkv 382 (612; both before the padding and the spill-free loop below, dq without the pass for D).  fp32: four, but one for up to
+// 32 rows, although the shapes of more than 64 columns spill there (hd 128: up to 173 / 255 / 495 registers): 64 sequences of one token on up to 3136 keys, hd 64
+// 70 us (four: 136), hd 80 169 (202), hd 128 290 (346); 512 pairs of 20 rows on 20 keys, hd 128 fwd 22.9 (22.8), dq 40 (29), dkv 40 (38), hd 64 9.0 (9.2), 12.2
+// (11.3), 11.3 (18.4).  bf16, hd 128, 4096 rows on 30 keys (one wave, rows in ranges, 278 spilled): dkv 48 us and two sums of 4.6.
 int row_waves(const dh_xattn_args* a, Kind kind, int64_t rows, int64_t other) {
   if (rows <= 32) return 1;
   if (a->dtype == DH_F32) return 4;
@@ -888,7 +897,8 @@ Plan plan_of(const dh_xattn_args* a, Kind kind, int64_t rows, int64_t other, int
   r.rw = row_waves(a, kind, rows, other);
   r.tiles = (int)cdiv64(rows < 1 ? 1 : rows, 32 * r.rw);
   // Two waves per SIMD; the forward of up to 64 columns fits three, and with ranges of 1024 keys and more their partial results cost less than they
-  // bring (24 pairs of 2047 on 6272: 161 us whole, 111 + 10 us in two ranges).
+  // bring (24 pairs of 2047 on 6272: 161 us whole, 104 + 9 us in two ranges).  That is 384 blocks, the most that still split; 48 and 96 pairs run whole, two
+  // waves per SIMD, in 280-297 and 445 us.
   const bool three = kind == FWD && a->dtype == DH_BF16 && a->hd <= 64 && r.rw == 4 && other >= 2048;
   const int64_t blocks = (int64_t)r.tiles * a->batch * a->kv_heads, want = (int64_t)x_cus() * ((three ? 12 : 8) / r.rw);
   if (three) step = 1024;

@@ -203,8 +203,8 @@ int dh_attn_pooled_bwd(int dtype, const void* q, const void* kv, const void* dou
  *   max_q / max_kv: longest query / key row count of a sequence as far as the caller knows it (0: unknown), used to lay out the grid only --
  *   longer sequences are computed whole.  Table entries are clamped to the row counts, so no table makes a kernel leave its buffers.
  *   scale > 0.  bf16: P and dS are rounded to bf16 as MFMA operands; statistics, sums and accumulators fp32.  No atomics: the same bits on every run.
- * fwd reads q k v, writes out lse; bwd reads q k v dout lse (fp32: out too; bf16 forms sum(do out) from unrounded values), writes dq dk dv.  ws: dh_xattn_ws_bytes(args, backward) bytes of scratch, 16-byte
- * aligned, not shared with anything that may run at the same time. */
+ * fwd reads q k v, writes out lse; bwd reads q k v dout lse (fp32: out too; bf16 forms sum(do out) from unrounded values), writes dq dk dv.
+ * ws: dh_xattn_ws_bytes(args, backward) bytes of scratch, 16-byte aligned, not shared with anything that may run at the same time. */
 typedef struct {
   int dtype, batch, heads, kv_heads, hd;
   int rows_q, rows_kv, max_q, max_kv;
@@ -255,7 +255,8 @@ int dh_rope_axes(const dh_rope_plan* plan, int dtype, const void* x, int64_t ldx
  * x, y, x_out, n, dx_out, dn, dx, dy [rows][d] contiguous, rows < 2^30, d <= 8192, gate vectors < 2^22; 16-byte accesses where d % 8 == 0 and the addresses allow it.
  * stats [4][rows] fp32: mean / rstd of both norms, written by fwd, read by bwd.  n is computed from x_out before its rounding to dtype.
  * bwd: dx_out and dn are the gradients of the two outputs (one may be NULL); parameter gradients are WRITTEN (not accumulated), fp32, NULL =
- * not wanted; ws: dh_join_norm_bwd_ws_bytes(args).  No atomics: the same bits on every run. */
+ * not wanted; ws: dh_join_norm_bwd_ws_bytes(args): 16 d bytes per block, of which there is at least one per gate vector (a vector per row: 16 bytes per
+ * element of x).  No atomics: the same bits on every run. */
 typedef struct {
   int dtype, rows, d;
   int rms, gate_rows, gate_channel, gate_tanh;
