@@ -20,7 +20,9 @@ def _rank(body, world, **env):
     env = dict({k: v for k, v in os.environ.items() if not k.startswith(("TORCHELASTIC", "DH_BENCH"))}, RANK="0", LOCAL_RANK="0", WORLD_SIZE=str(world),
                MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), DH_DIST_BACKEND="gloo", **env)
     code = "import sys, time; sys.path.insert(0, %r); import bench; sys.argv = ['bench.py', '--dry-run-launch', '--gpus', '%d', '--graph', '1']\n%s" % (ROOT, world, body)
-    return subprocess.Popen([sys.executable, "-u", "-c", code], env=env, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True, cwd=ROOT)
+    p = subprocess.Popen([sys.executable, "-u", "-c", code], env=env, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True, cwd=ROOT)
+    p.port = port + 1                                # where its second attempt listens
+    return p
 
 
 def _children(pid):
@@ -59,20 +61,17 @@ def test_the_second_attempt_speaks_for_the_rank():
 @pytest.mark.parametrize("ready", [False, True])
 def test_the_second_attempt_ends_with_its_rank(sig, ready):
     """a launcher that terminates or kills the rank knows one process: the attempt under way (here it waits for a rank 1 that never comes) goes with it"""
-    p = _rank("bench._arm_watchdog(0.1, 'a step')\ntime.sleep(600)", 2)
+    p, kids = _rank("bench._arm_watchdog(0.1, 'a step')\ntime.sleep(600)", 2), []
     try:
         kids = _wait(lambda: _children(p.pid))
         assert len(kids) == 1
         if ready:                                    # (it listens for its peers: up and running)
-            port = None
-            with open("/proc/%d/environ" % kids[0]) as f:
-                port = int(dict(e.split("=", 1) for e in f.read().split("\0") if "=" in e)["MASTER_PORT"])
-            assert _wait(lambda: any(line.split()[1].endswith(":%04X" % port) and line.split()[3] == "0A" for t in ("tcp", "tcp6") for line in open("/proc/net/" + t).readlines()[1:]))
+            assert _wait(lambda: any(line.split()[1].endswith(":%04X" % p.port) and line.split()[3] == "0A" for t in ("tcp", "tcp6") for line in open("/proc/net/" + t).readlines()[1:]))
         p.send_signal(sig)
         p.wait(30)
         assert _wait(lambda: not _alive(kids[0]), 60), "the second attempt outlived its rank"
     finally:
-        for pid in [p.pid] + (kids if "kids" in locals() else []):
+        for pid in [p.pid] + kids:
             try:
                 os.kill(pid, signal.SIGKILL)
             except OSError:
