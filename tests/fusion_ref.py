@@ -22,12 +22,8 @@ def lengths(cu, rows, batch):
     return [(int(cu[i]), int(cu[i + 1]) - int(cu[i])) for i in range(batch)]
 
 
-def xattn(q, k, v, heads, dout=None, kv_heads=None, batch=None, cu_q=None, cu_kv=None, kv_len=None, key_mask=None, scale=None, norms=None):
-    """{name: (value, bound)} of out, lse (, dq, dk, dv).
-    norms (a dict): filled with the norm that the error of dq / dk may have.  Relative roundings spread over at most [-u, u] have a mean square of u^2 / 3 at
-    most, independent ones add up in squares, and the norm of a few hundred of them stays within 15 % of that: dS is rounded to the operand type element
-    by element, the result once more.  fp32's roundings are counted the same way (a sum of n products: sqrt(n / 3) UF of the magnitudes), twice what they
-    come to; what moves a whole row (D = sum p dp from unrounded p and dp, lse) is added up before it is squared."""
+def xattn(q, k, v, heads, dout=None, kv_heads=None, batch=None, cu_q=None, cu_kv=None, kv_len=None, key_mask=None, scale=None):
+    """{name: (value, bound)} of out, lse (, dq, dk, dv)"""
     u = unit(q.dtype)
     up = u if q.dtype == torch.bfloat16 else 0.0
     kv_heads = kv_heads or heads
@@ -39,8 +35,6 @@ def xattn(q, k, v, heads, dout=None, kv_heads=None, batch=None, cu_q=None, cu_kv
     lse, el = torch.full((heads, q.shape[0]), -math.inf, dtype=F64), z(heads, q.shape[0])
     dq, edq = z(q.shape[0], heads, hd), z(q.shape[0], heads, hd)
     dk, edk, dv, edv = (z(k.shape[0], kv_heads, hd) for _ in range(4))
-    if norms is not None:
-        sq, fine = {"dq": 0.0, "dk": 0.0}, {"dq": 0.0, "dk": 0.0}
     for i, ((q0, nq), (k0, nk)) in enumerate(zip(lengths(cu_q, q.shape[0], batch), lengths(cu_kv, k.shape[0], batch))):
         if kv_len is not None:
             nk = min(nk, max(int(kv_len[i]), 0))
@@ -80,23 +74,11 @@ def xattn(q, k, v, heads, dout=None, kv_heads=None, batch=None, cu_q=None, cu_kv
             edq[rows, h] = scale * (eds @ K.abs() + n * UF * (ds.abs() @ K.abs())) + u * dq[rows, h].abs()
             dk[keys, g] += scale * (ds.T @ Q)
             edk[keys, g] += scale * (eds.T @ Q.abs() + nq * rep * UF * (ds.abs().T @ Q.abs()))
-            if norms is not None:
-                sq["dq"] += float(((scale * ds) ** 2 @ (K * K)).sum())
-                sq["dk"] += float(((scale * ds).T ** 2 @ (Q * Q)).sum())
-                one = scale * (Q.abs() @ K.abs().T) * math.sqrt((hd + 4) / 3) * UF + 4 * UF * s.abs()
-                whole = (P * one).sum(1, keepdim=True) + (math.sqrt(n) + 16) * UF + 8 * UF * (1 + L.abs()[:, None])
-                e1 = P * (do.abs() @ V.abs().T) * math.sqrt((hd + 2) / 3) * UF + (one + whole + 4 * UF) * ds.abs()
-                e2 = (P * ((do.abs() @ V.abs().T) * math.sqrt((hd + 2) / 3) * UF + (one + whole + math.sqrt(n / 3) * UF) * dp.abs())).sum(1, keepdim=True)
-                fine["dq"] += scale ** 2 * float((e1 ** 2 @ (K * K) + (e2 * (P @ K)) ** 2 + n * UF ** 2 * (ds ** 2 @ (K * K))).sum())
-                fine["dk"] += scale ** 2 * float(((e1 + P * e2).T ** 2 @ (Q * Q) + nq * rep * UF ** 2 * (ds.T ** 2 @ (Q * Q))).sum())
             dv[keys, g] += P.T @ do
             edv[keys, g] += ((rp + up).expand_as(P) * P).T @ do.abs() + nq * rep * UF * (P.T @ do.abs())
     flat = lambda t: t.reshape(t.shape[0], -1)  # noqa: E731
     res = {"out": (flat(out), flat(eo)), "lse": (lse, el)}
     if dout is not None:
-        if norms is not None:
-            for name, t in (("dq", dq), ("dk", dk)):
-                norms[name] = 1.15 * u / math.sqrt(3) * math.sqrt((sq[name] if up else 0.0) + float((t * t).sum())) + 2 * math.sqrt(fine[name])
         res.update(dq=(flat(dq), flat(edq)), dk=(flat(dk), flat(edk) + u * flat(dk).abs()), dv=(flat(dv), flat(edv) + u * flat(dv).abs()))
     return res
 

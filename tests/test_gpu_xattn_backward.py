@@ -3,8 +3,8 @@ dS = p (dp - D) is then small beside dp and D, and an error of D shows in full."
 import pytest
 import torch
 
-import fusion_ref as R
 from test_gpu_fusion import dev, geometry, rnd
+from xattn_norms import gradients
 
 pytestmark = pytest.mark.gpu
 
@@ -19,15 +19,15 @@ def run(dtype, heads, kv_heads, hd, rows_q, rows_kv, kw, sharp, mask=None):
     kw = dict(kw, kv_heads=kv_heads)
     if mask is not None:
         kw["key_mask"] = mask
-    norms = {}
-    ref = R.xattn(q, k, v, heads, dout, norms=norms, **kw)
+    ref = gradients(q, k, v, heads, dout, **kw)
     args = {n: dev(t) for n, t in kw.items()}
     qd, kd, vd = q.to(cuda), k.to(cuda), v.to(cuda)
     out, lse = ops.xattn_fwd(qd, kd, vd, heads, **args)
     dq, dk, dv = ops.xattn_bwd(qd, kd, vd, out, dout.to(cuda), lse, heads, **args)
     for name, t in (("dq", dq), ("dk", dk)):
-        off = float((t.cpu().double() - ref[name][0]).norm())
-        assert off <= norms[name], "%s: off by %.3g of its norm, %.3g allowed" % (name, off / float(ref[name][0].norm()), norms[name] / float(ref[name][0].norm()))
+        value, allowed = ref[name]
+        off, size = float((t.cpu().double() - value).norm()), float(value.norm())
+        assert off <= allowed, "%s: off by %.3g of its norm, %.3g allowed" % (name, off / size, allowed / size)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
